@@ -47,6 +47,20 @@ if _calls is not None:
     _calls.setup(c_ptr, WeightRef)
 
 
+class KvCacheStruct(ctypes.Structure):
+    """lx_b200_kv_cache of include/dromos_b200.h: a host struct whose pointers are device pointers."""
+
+    _fields_ = [("type", c_int), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page_tokens", ctypes.c_int32), ("pages", c_i64),
+                ("page_stride", c_i64), ("k", c_ptr), ("v", c_ptr), ("k_scale", c_ptr), ("v_scale", c_ptr)]
+
+
+class KvBatchStruct(ctypes.Structure):
+    """lx_b200_kv_batch of include/dromos_b200.h."""
+
+    _fields_ = [("sequences", ctypes.c_int32), ("tokens", ctypes.c_int32), ("max_new", ctypes.c_int32), ("ld_pages", ctypes.c_int32), ("starts", c_ptr),
+                ("lengths", c_ptr), ("pages", c_ptr)]
+
+
 class LxTuneProblem(ctypes.Structure):
     """lx_tune_problem (engine/cuda/tunable.h:57-62)."""
 
@@ -120,6 +134,16 @@ EXTENSIONS = {
     "lx_b200_moe_exchange_rows": (c_int, [c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_int, c_int, c_ptr, c_int, c_int, c_int, c_int, c_int, c_ptr]),
     "lx_b200_moe_sum_rows": (c_int, [c_ptr, c_ptr, c_int, c_int, c_int, c_ptr]),
     "lx_b200_exchange_packets": (c_int, [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_int, c_int, c_ptr, c_int, c_int, c_int, c_ptr]),
+    # cache, batch, k, ld_k, v, ld_v, kv_dtype, q, q_dtype, ld_q, q_heads, q_out, q_out_dtype, ld_q_out, positions, frequencies, rotary_dim, interleaved, stream
+    "lx_b200_kv_append": (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_int, c_int, c_ptr, c_int, c_int, c_int, c_ptr, c_int, c_int, c_ptr, c_ptr, c_int,
+                                  c_int, c_ptr]),
+    # cache, batch, q, q_dtype, ld_q, q_heads, scale, window, out, ld_out, workspace, stream
+    "lx_b200_attention": (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_f32, c_int, c_ptr, c_int, c_ptr, c_ptr]),
+    "lx_b200_attention_workspace_bytes": (c_i64, [c_ptr, c_int, c_int]),
+    # y, y_dtype, ld_y, h, h_dtype, ld_h, gate, gate_dtype, ld_gate, gate_sigmoid, post, pre, weight_dtype, residual_scale, block_scale, eps, h_out, ld_h_out,
+    # x, x_dtype, ld_x, T, C, stream
+    "lx_b200_norm_residual": (c_int, [c_ptr, c_int, c_int, c_ptr, c_int, c_int, c_ptr, c_int, c_int, c_int, c_ptr, c_ptr, c_int, c_f32, c_f32, c_f32, c_ptr,
+                                      c_int, c_ptr, c_int, c_int, c_int, c_int, c_ptr]),
 }
 ERR_SCRATCH = 804
 

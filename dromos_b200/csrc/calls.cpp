@@ -124,6 +124,10 @@ const Entry kEntries[] = {
     ENTRY(lx_moe_grouped_workspace_bytes),
     ENTRY(lx_moe_experts_decode),
     ENTRY(lx_moe_decode_workspace_bytes),
+    ENTRY(lx_b200_kv_append),
+    ENTRY(lx_b200_attention),
+    ENTRY(lx_b200_attention_workspace_bytes),
+    ENTRY(lx_b200_norm_residual),
 };
 #undef ENTRY
 

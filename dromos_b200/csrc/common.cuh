@@ -23,6 +23,7 @@ constexpr int kStatusFullWait = 1;   // a consumer waited for a weight stage tha
 constexpr int kStatusEmptyWait = 2;  // the producer waited for a ring slot that was never released
 constexpr int kStatusDrainWait = 3;  // the final drain of in-flight copies ran out
 constexpr int kStatusPartWait = 4;   // a CTA waited for another CTA's partial sums that never came
+constexpr int kStatusBatch = 9;      // a batch of cached sequences named rows, pages or lengths that cannot be
 
 // ---- host: launch accounting and status -----------------------------------------------------------------
 extern std::atomic<int64_t> g_launches;

@@ -1,0 +1,72 @@
+// The paged 8-bit cache of keys and values as its kernels see it: arguments, checks of them, the rule of its scales.
+#pragma once
+
+#include <climits>
+
+#include "launch.cuh"
+
+namespace b200 {
+namespace {
+
+// Smallest and largest exponent of a scale the append writes. The lower end keeps the sum of a softmax's weights, which are
+// held divided by these scales, inside f32: 2^100 times a million tokens is 2^120. No f32 needs one above the upper end.
+constexpr int kScaleMin = -100, kScaleMax = 122;
+
+struct KvView {
+  uint8_t *k, *v;
+  float *k_scale, *v_scale;
+  int64_t pages, page_stride;
+  int kv_heads, page_tokens;
+  const int32_t *starts, *lengths, *table;
+  int sequences, tokens, ld_pages;
+  int* status;
+};
+
+// A sequence's rows and slots, 0 new tokens where what the arrays say cannot be.
+struct Span {
+  int row0, n, length;
+};
+__device__ __forceinline__ Span span_of(const KvView& A, int s, bool& bad) {
+  const int r0 = A.starts[s], r1 = A.starts[s + 1], len = A.lengths[s];
+  bad = r0 < 0 || r1 < r0 || r1 > A.tokens || len < 0;
+  return bad ? Span{0, 0, 0} : Span{r0, r1 - r0, len};
+}
+// The page that holds a sequence's slots page_tokens * i and on, or -1.
+__device__ __forceinline__ int page_of(const KvView& A, int s, int i) {
+  if (i < 0 || i >= A.ld_pages) return -1;
+  const int p = A.table[static_cast<int64_t>(s) * A.ld_pages + i];
+  return p < 0 || p >= A.pages ? -1 : p;
+}
+__device__ __forceinline__ void report_batch(const KvView& A) {
+  if (A.status) atomicExch(A.status, kStatusBatch);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+inline int check_cache(const lx_b200_kv_cache* c) {
+  if (!c || c->kv_heads < 1 || c->pages < 1 || !c->k || !c->v || !c->k_scale || !c->v_scale) return kInvalid;
+  if (c->type != LX_W_FP8 && c->type != LX_W_INT8) return kNotSupported;
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return kNotSupported;
+  if (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128) return kNotSupported;
+  if (c->kv_heads > 1024 || c->pages > INT_MAX) return kNotSupported;
+  const int64_t page = static_cast<int64_t>(c->kv_heads) * c->page_tokens * c->head_dim;
+  if (c->page_stride < page || c->page_stride % 16 || !aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
+    return kInvalid;
+  return kOk;
+}
+inline int check_batch(const lx_b200_kv_batch* b) {
+  if (!b || b->sequences < 0 || b->tokens < 0 || b->max_new < 0 || b->ld_pages < 0) return kInvalid;
+  if (b->sequences > 0 && (!b->starts || !b->lengths || (b->ld_pages > 0 && !b->pages))) return kInvalid;
+  return kOk;
+}
+inline KvView view_of(const lx_b200_kv_cache& c, const lx_b200_kv_batch& b) {
+  KvView A;
+  A.k = static_cast<uint8_t*>(c.k), A.v = static_cast<uint8_t*>(c.v), A.k_scale = c.k_scale, A.v_scale = c.v_scale;
+  A.pages = c.pages, A.page_stride = c.page_stride, A.kv_heads = c.kv_heads, A.page_tokens = c.page_tokens;
+  A.starts = b.starts, A.lengths = b.lengths, A.table = b.pages;
+  A.sequences = b.sequences, A.tokens = b.tokens, A.ld_pages = b.ld_pages;
+  A.status = status_word();
+  return A;
+}
+
+}  // namespace
+}  // namespace b200

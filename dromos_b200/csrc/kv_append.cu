@@ -1,0 +1,244 @@
+// lx_b200_kv_append: new keys and values into a paged 8-bit cache, rotated on the way, and the rotated queries.
+//
+// A CTA has the new tokens of one page for one key head: it alone decides the page's scales for that head, so there are no atomics and
+// the codes do not depend on the order of anything. It reads its rows twice: once for their largest magnitudes, once (from the
+// caches) for their codes.
+#include <algorithm>
+
+#include "kv.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kAppendThreads = 256;
+constexpr int kAnglePairs = 4096;  // cosines and sines held at once: 32 KB
+
+struct AppendArgs {
+  KvView kv;
+  const void *k, *v, *q;
+  void* q_out;
+  int64_t ld_k, ld_v, ld_q, ld_q_out;
+  int kv_dtype, q_dtype, q_out_dtype, group, head_dim, rotary, interleaved, int8, splits;
+  bool k_vec, v_vec, q_vec, q_out_vec;  // rows in whole pieces of four values
+  const int32_t* positions;
+  const double* frequencies;
+};
+
+__device__ __forceinline__ float4 load4(const void* p, int dtype, int64_t i, bool vec) {
+  if (vec) {
+    if (dtype == LX_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+  }
+  return make_float4(load_f32(p, dtype, i), load_f32(p, dtype, i + 1), load_f32(p, dtype, i + 2), load_f32(p, dtype, i + 3));
+}
+__device__ __forceinline__ void store4(void* p, int dtype, int64_t i, const float* v, bool vec) {
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) store_from_f32(p, dtype, i + j, v[j]);
+  } else if (dtype == LX_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) =
+        make_uint2(f32_to_bf16_bits(v[0]) | f32_to_bf16_bits(v[1]) << 16, f32_to_bf16_bits(v[2]) | f32_to_bf16_bits(v[3]) << 16);
+  }
+}
+
+// A piece of a head is eight values that turn together: two runs of four, `first` and `second`, that begin at lo and hi.
+struct Piece {
+  int lo, hi, pair;  // pair: the first of its four pairs, -1 where nothing turns
+};
+__device__ __forceinline__ Piece piece_of(const AppendArgs& A, int u) {
+  const int r = A.rotary;
+  if (8 * u >= r) return {8 * u, 8 * u + 4, -1};
+  return A.interleaved ? Piece{8 * u, 8 * u + 4, 4 * u} : Piece{4 * u, 4 * u + r / 2, 4 * u};
+}
+// The eight values of a piece, turned by the angles at cs.
+__device__ __forceinline__ void load_piece(const AppendArgs& A, const void* p, int dtype, int64_t head, const Piece& u, bool vec, const float2* cs, float (&x)[8]) {
+  const float4 a = load4(p, dtype, head + u.lo, vec), b = load4(p, dtype, head + u.hi, vec);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  if (u.pair < 0 || !cs) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i0 = A.interleaved ? 2 * j : j, i1 = A.interleaved ? 2 * j + 1 : j + 4;
+    const float2 c = cs[u.pair + j];
+    const float s = x[i0], t = x[i1];
+    x[i0] = s * c.x - t * c.y;
+    x[i1] = t * c.x + s * c.y;
+  }
+}
+// Four codes of values already divided by their scale.
+__device__ __forceinline__ uint32_t codes4(const float* v, int int8) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t b = int8 ? static_cast<uint32_t>(static_cast<int>(rintf(fminf(fmaxf(v[j], -127.0f), 127.0f)))) & 0xffu : e4m3_encode(v[j]) & 0xffu;
+    w |= b << (8 * j);
+  }
+  return w;
+}
+// The smallest power of two, within the limits, that brings a magnitude (its bits) to 448 (0.875 * 2^9) or 127 ((1 - 2^-7) * 2^7) or less.
+__device__ __forceinline__ float scale_for(uint32_t magnitude, int int8) {
+  if (magnitude >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
+  if (magnitude < 0x00800000u) return __uint_as_float(static_cast<uint32_t>(127 + kScaleMin) << 23);
+  const int e = static_cast<int>(magnitude >> 23) - 126;  // magnitude = m 2^e, m in [0.5, 1)
+  const uint32_t m = magnitude & 0x7fffffu;
+  const int want = int8 ? e - 7 + (m > 0x7e0000u) : e - 9 + (m > 0x600000u);
+  return __uint_as_float(static_cast<uint32_t>(127 + min(max(want, kScaleMin), kScaleMax)) << 23);
+}
+
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendArgs A) {
+  __shared__ float2 angles[kAnglePairs];
+  __shared__ uint32_t most[2];
+  pdl_wait();
+  const KvView& C = A.kv;
+  const int s = blockIdx.x / A.splits, head = blockIdx.y, tid = threadIdx.x;
+  bool bad;
+  const Span q = span_of(C, s, bad);
+  bad = bad || q.length < q.n;
+  if (bad) {
+    if (tid == 0 && head == 0) report_batch(C);
+    return;
+  }
+  if (q.n == 0) return;
+  const int P = C.page_tokens, D = A.head_dim, units = D / 8, first = q.length - q.n, half = A.rotary / 2;
+  const int chunk = half ? min(P, kAnglePairs / half) : P;
+  for (int page = first / P + blockIdx.x % A.splits; page <= (q.length - 1) / P; page += A.splits) {
+    const int lo = max(first, page * P), n = min(q.length, page * P + P) - lo, row0 = q.row0 + lo - first, kept = lo - page * P;
+    const int at = page_of(C, s, page);
+    if (at < 0 && tid == 0 && head == 0) report_batch(C);
+    if (tid < 2) most[tid] = 0;
+    float now[2], inverse[2];
+    for (int pass = 0; pass < 2; ++pass) {
+      uint32_t large[2] = {0, 0};
+      for (int c0 = 0; c0 < n; c0 += chunk) {
+        const int m = min(chunk, n - c0);
+        __syncthreads();  // whoever still reads the angles, or `most`
+        if (half && (pass == 0 || n > chunk))
+          for (int i = tid; i < m * half; i += kAppendThreads) {
+            const int t = i / half;
+            const int position = A.positions ? A.positions[row0 + c0 + t] : lo + c0 + t;
+            // in turns, less the whole ones, before anything is rounded to f32: a position of a million costs no digits
+            double turns = static_cast<double>(position) * A.frequencies[i - t * half] * 0.15915494309189533577;
+            turns -= rint(turns);
+            float2 cs;
+            sincospif(2.0f * static_cast<float>(turns), &cs.y, &cs.x);
+            angles[i] = cs;
+          }
+        __syncthreads();
+        const float2* cs = half ? angles : nullptr;
+        for (int i = tid; i < m * units; i += kAppendThreads) {
+          const int t = i / units;
+          const Piece u = piece_of(A, i - t * units);
+          float x[8], y[8];
+          load_piece(A, A.k, A.kv_dtype, (row0 + c0 + t) * A.ld_k + head * D, u, A.k_vec, cs + t * half, x);
+          load_piece(A, A.v, A.kv_dtype, (row0 + c0 + t) * A.ld_v + head * D, u, A.v_vec, nullptr, y);
+          if (pass == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              large[0] = max(large[0], __float_as_uint(x[j]) & 0x7fffffffu);  // as integers: not-a-number is the largest
+              large[1] = max(large[1], __float_as_uint(y[j]) & 0x7fffffffu);
+            }
+          } else if (at >= 0) {
+            const int64_t dst = at * C.page_stride + (static_cast<int64_t>(head) * P + kept + c0 + t) * D;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = now[0] == now[0] ? x[j] * inverse[0] : 0.0f, y[j] = now[1] == now[1] ? y[j] * inverse[1] : 0.0f;
+            *reinterpret_cast<uint32_t*>(C.k + dst + u.lo) = codes4(x, A.int8);
+            *reinterpret_cast<uint32_t*>(C.k + dst + u.hi) = codes4(x + 4, A.int8);
+            *reinterpret_cast<uint32_t*>(C.v + dst + u.lo) = codes4(y, A.int8);
+            *reinterpret_cast<uint32_t*>(C.v + dst + u.hi) = codes4(y + 4, A.int8);
+          }
+        }
+        if (pass == 0)
+          for (int i = tid; i < m * A.group * units; i += kAppendThreads) {
+            const int t = i / (A.group * units), g = (i / units) % A.group;
+            const Piece u = piece_of(A, i % units);
+            float x[8];
+            const int64_t col = static_cast<int64_t>(head * A.group + g) * D;
+            load_piece(A, A.q, A.q_dtype, (row0 + c0 + t) * A.ld_q + col, u, A.q_vec, cs + t * half, x);
+            store4(A.q_out, A.q_out_dtype, (row0 + c0 + t) * A.ld_q_out + col + u.lo, x, A.q_out_vec);
+            store4(A.q_out, A.q_out_dtype, (row0 + c0 + t) * A.ld_q_out + col + u.hi, x + 4, A.q_out_vec);
+          }
+      }
+      if (pass == 0) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          large[w] = __reduce_max_sync(0xffffffffu, large[w]);
+          if ((tid & 31) == 0) atomicMax(&most[w], large[w]);
+        }
+        __syncthreads();
+        if (at < 0) break;
+        const int64_t sc = static_cast<int64_t>(at) * C.kv_heads + head;
+        float* const scales[2] = {C.k_scale + sc, C.v_scale + sc};
+        uint8_t* const codes[2] = {C.k, C.v};
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const float want = scale_for(most[w], A.int8), was = kept ? *scales[w] : want;
+          // not-a-number, of old or of new values, stays
+          now[w] = was != was || want != want ? __uint_as_float(0x7fffffffu) : fmaxf(was, want);
+          inverse[w] = 1.0f / now[w];
+          if (kept && now[w] > was) {
+            const float ratio = was / now[w];
+            uint4* held = reinterpret_cast<uint4*>(codes[w] + at * C.page_stride + static_cast<int64_t>(head) * P * D);
+            for (int i = tid; i < kept * D / 16; i += kAppendThreads) {
+              const uint4 old = held[i];
+              uint32_t word[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const uint32_t code = word[b] >> (8 * j) & 0xffu;
+                  x[j] = (A.int8 ? static_cast<float>(static_cast<int8_t>(code)) : (code & 0x7fu) == 0x7fu ? __uint_as_float(0x7fffffffu) : e4m3_to_f32(code)) * ratio;
+                }
+                word[b] = codes4(x, A.int8);
+              }
+              held[i] = make_uint4(word[0], word[1], word[2], word[3]);
+            }
+          }
+        }
+        __syncthreads();  // every thread has read the old scales
+        if (tid < 2) *scales[tid] = now[tid];
+      }
+    }
+    __syncthreads();  // before `most` starts anew
+  }
+}
+
+// Whether rows of heads begin and go on in pieces of four values.
+bool fours(const void* p, int dtype, int64_t ld) { return aligned(p, dtype == LX_BF16 ? 8 : 16) && ld % 4 == 0; }
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int lx_b200_kv_append(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* k, int ld_k, const void* v, int ld_v,
+                                 lx_dtype kv_dtype, const void* q, lx_dtype q_dtype, int ld_q, int q_heads, void* q_out, lx_dtype q_out_dtype,
+                                 int ld_q_out, const int32_t* positions, const double* frequencies, int rotary_dim, int interleaved,
+                                 void* stream) {
+  if (int e = check_cache(cache)) return e;
+  if (int e = check_batch(batch)) return e;
+  const int64_t D = cache->head_dim, H = cache->kv_heads;
+  if (!valid_dtype(kv_dtype) || !valid_dtype(q_dtype) || !valid_dtype(q_out_dtype) || q_heads < 0 || rotary_dim < 0 || rotary_dim > D) return kInvalid;
+  if (rotary_dim % 8) return kNotSupported;
+  if (rotary_dim && !frequencies) return kInvalid;
+  if (batch->sequences == 0 || batch->tokens == 0) return kOk;
+  if (!k || !v || ld_k < H * D || ld_v < H * D) return kInvalid;
+  const int heads = q ? q_heads : 0;
+  if (q && (q_heads < 1 || q_heads % H || !q_out || ld_q < q_heads * D || ld_q_out < q_heads * D)) return kInvalid;
+  AppendArgs A;
+  A.kv = view_of(*cache, *batch);
+  A.k = k, A.v = v, A.q = q, A.q_out = q_out;
+  A.ld_k = ld_k, A.ld_v = ld_v, A.ld_q = ld_q, A.ld_q_out = ld_q_out;
+  A.kv_dtype = kv_dtype, A.q_dtype = q_dtype, A.q_out_dtype = q_out_dtype;
+  A.group = heads / static_cast<int>(H), A.head_dim = static_cast<int>(D), A.rotary = rotary_dim, A.interleaved = interleaved;
+  A.int8 = cache->type == LX_W_INT8;
+  A.k_vec = fours(k, kv_dtype, ld_k), A.v_vec = fours(v, kv_dtype, ld_v), A.q_vec = fours(q, q_dtype, ld_q), A.q_out_vec = fours(q_out, q_out_dtype, ld_q_out);
+  A.positions = positions, A.frequencies = frequencies;
+  // CTAs per sequence and head: as many pages as max_new tokens reach at most (a sequence with more: its CTAs take several)
+  const int P = cache->page_tokens, most = std::min(std::max(batch->max_new, 1), batch->tokens);
+  A.splits = (most + P - 2) / P + 1;
+  return launch_kernel(kv_append_kernel, dim3(static_cast<unsigned>(batch->sequences) * A.splits, static_cast<unsigned>(H)), dim3(kAppendThreads), 0,
+                       static_cast<cudaStream_t>(stream), A);
+}

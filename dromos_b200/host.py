@@ -222,6 +222,235 @@ class Experts:
         return out
 
 
+def _dtype(x: torch.Tensor, what: str) -> int:
+    if x.dtype == torch.bfloat16:
+        return abi.BF16
+    if x.dtype == torch.float32:
+        return abi.F32
+    raise TypeError(f"{what}: bfloat16 or float32, not {x.dtype}")
+
+
+def _rows(x: torch.Tensor, rows: int, cols: int, what: str, device=None) -> int:
+    """The row stride of a [rows, cols] tensor whose rows are contiguous."""
+    if x.dim() != 2 or x.shape[0] != rows or x.shape[1] != cols or (cols > 1 and x.stride(1) != 1):
+        raise ValueError(f"{what}: [{rows}, {cols}] with contiguous rows, not {tuple(x.shape)} with strides {x.stride()}")
+    if device is not None and x.device != device:
+        raise ValueError(f"{what} is on {x.device}, the call on {device}")
+    return x.stride(0) if rows > 1 else max(cols, x.stride(0))
+
+
+def _here(device: torch.device):
+    """Calls launch on the current device's current stream: a buffer of another device is refused, not touched."""
+    if device.type != "cuda":
+        raise ValueError(f"the buffers are on {device}, not on a CUDA device")
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"the buffers are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+class Rotary:
+    """The rotation of positions: frequencies f64 [rotary_dim / 2] (radians per position), the pairs they turn."""
+
+    def __init__(self, frequencies: torch.Tensor, interleaved: bool = False):
+        if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
+            raise ValueError("frequencies: a contiguous float64 vector")
+        self.frequencies, self.interleaved, self.dim = frequencies, interleaved, 2 * frequencies.numel()
+
+    @classmethod
+    def of(cls, dim: int, base: float = 10000.0, device="cuda", interleaved: bool = False):
+        return cls(torch.pow(torch.tensor(base, dtype=torch.float64), -torch.arange(0, dim, 2, dtype=torch.float64) / dim).to(device), interleaved)
+
+
+class KvBatch:
+    """The sequences of a call: starts int32 [S + 1] (sequence s has the rows starts[s] .. starts[s + 1] - 1, its new tokens), lengths
+    int32 [S] (its tokens in the cache with these), pages int32 [S, n] (its pages in order). All three stay on the device and are
+    read when the kernels run, so a captured call follows what is written to them. tokens: rows of the call's buffers; max_new: the
+    most new tokens of one sequence, a hint."""
+
+    def __init__(self, starts: torch.Tensor, lengths: torch.Tensor, pages: torch.Tensor, tokens: int, max_new: int):
+        S = lengths.shape[0]
+        for x, shape, what in ((starts, (S + 1,), "starts"), (lengths, (S,), "lengths")):
+            if x.dtype != torch.int32 or tuple(x.shape) != shape or not x.is_contiguous():
+                raise ValueError(f"{what}: contiguous int32 {shape}, not {x.dtype} {tuple(x.shape)}")
+        if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != S or not pages.is_contiguous():
+            raise ValueError(f"pages: contiguous int32 [{S}, n], not {pages.dtype} {tuple(pages.shape)}")
+        if starts.device != lengths.device or pages.device != lengths.device:
+            raise ValueError("starts, lengths and pages on one device")
+        if tokens < 0 or max_new < 0:
+            raise ValueError("tokens and max_new count from 0")
+        self.starts, self.lengths, self.pages, self.tokens, self.max_new = starts, lengths, pages, tokens, max_new
+        self.device = lengths.device
+        self.struct = abi.KvBatchStruct(S, tokens, max_new, pages.shape[1], starts.data_ptr(), lengths.data_ptr(), pages.data_ptr())
+        self.address = ctypes.addressof(self.struct)
+
+
+class KvCache:
+    """A paged cache of keys and values in 8 bits (lx_b200_kv_cache): codes uint8 [pages, kv_heads, page_tokens, head_dim] for each, E4M3
+    (abi.W_FP8) or signed bytes (abi.W_INT8), the stride between pages free; scales f32 [pages, kv_heads]."""
+
+    def __init__(self, lib, wtype: int, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        pages, heads, P, D = k.shape
+        for x, what in ((k, "k"), (v, "v")):
+            if x.element_size() != 1 or x.shape != k.shape or x.stride()[1:] != (P * D, D, 1) or x.stride(0) != k.stride(0):
+                raise ValueError(f"{what}: 8-bit [pages, heads, page_tokens, head_dim], contiguous within a page, k and v alike")
+        for x, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if x.dtype != torch.float32 or tuple(x.shape) != (pages, heads) or not x.is_contiguous():
+                raise ValueError(f"{what}: contiguous float32 [{pages}, {heads}], not {x.dtype} {tuple(x.shape)}")
+        if any(x.device != k.device for x in (v, k_scale, v_scale)):
+            raise ValueError("codes and scales on one device")
+        self.lib, self.wtype, self.k, self.v, self.k_scale, self.v_scale = lib, wtype, k, v, k_scale, v_scale
+        self.pages, self.kv_heads, self.page_tokens, self.head_dim, self.device = pages, heads, P, D, k.device
+        stride = k.stride(0) if pages > 1 else heads * P * D
+        self.struct = abi.KvCacheStruct(wtype, heads, D, P, pages, stride, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        self.address = ctypes.addressof(self.struct)
+
+    @classmethod
+    def empty(cls, lib, wtype: int, pages: int, kv_heads: int, head_dim: int, page_tokens: int = 64, device="cuda"):
+        codes = [torch.zeros((pages, kv_heads, page_tokens, head_dim), dtype=torch.uint8, device=device) for _ in range(2)]
+        scales = [torch.ones((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(lib, wtype, *codes, *scales)
+
+    def append(self, batch: KvBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, rotary: Rotary | None = None,
+               positions: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+        """Writes the batch's new tokens, k and v [tokens, kv_heads * head_dim], to its pages, keys turned by `rotary`; returns the queries
+        q [tokens, heads * head_dim] turned the same way (bf16 where q_out does not say otherwise), None without q."""
+        T, width = batch.tokens, self.kv_heads * self.head_dim
+        _here(self.device)
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
+        ld_k, ld_v = _rows(k, T, width, "k", self.device), _rows(v, T, width, "v", self.device)
+        dt = _dtype(k, "k")
+        if v.dtype != k.dtype:
+            raise TypeError("k and v of one type")
+        heads = ld_q = ld_o = 0
+        q_dt = o_dt = abi.BF16
+        if q is not None:
+            heads = q.shape[1] // self.head_dim
+            ld_q, q_dt = _rows(q, T, heads * self.head_dim, "q", self.device), _dtype(q, "q")
+            if q_out is None:
+                q_out = torch.empty((T, heads * self.head_dim), dtype=torch.bfloat16, device=q.device)
+            ld_o, o_dt = _rows(q_out, T, heads * self.head_dim, "q_out", self.device), _dtype(q_out, "q_out")
+        if positions is not None and (positions.dtype != torch.int32 or tuple(positions.shape) != (T,) or not positions.is_contiguous() or positions.device != self.device):
+            raise ValueError(f"positions: contiguous int32 [{T}] on {self.device}")
+        if rotary is not None and rotary.frequencies.device != self.device:
+            raise ValueError(f"the frequencies are on {rotary.frequencies.device}, the cache on {self.device}")
+        st = self.lib.lx_b200_kv_append(self.address, batch.address, k.data_ptr(), ld_k, v.data_ptr(), ld_v, dt, q.data_ptr() if q is not None else None, q_dt,
+                                        ld_q, heads, q_out.data_ptr() if q is not None else None, o_dt, ld_o,
+                                        positions.data_ptr() if positions is not None else None, rotary.frequencies.data_ptr() if rotary is not None else None,
+                                        rotary.dim if rotary is not None else 0, int(rotary is not None and rotary.interleaved), _raw_stream())
+        if st:
+            raise RuntimeError(f"lx_b200_kv_append failed: {st}")
+        return q_out if q is not None else None
+
+
+class Attention:
+    """Causal attention of new tokens' queries over a cache. Each call takes its workspace from torch's allocator, so calls on several
+    streams and captured graphs share none."""
+
+    def __init__(self, cache: KvCache, heads: int, scale: float | None = None, window: int = 0):
+        self.cache, self.heads, self.window = cache, heads, window
+        self.scale = float(cache.head_dim**-0.5 if scale is None else scale)
+        self._need = {}  # by max_new
+        if cache.lib.lx_b200_attention_workspace_bytes(cache.address, heads, 1) < 0:
+            raise ValueError(f"no attention of {heads} heads over this cache")
+
+    def __call__(self, batch: KvBatch, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """q: f32 or bf16 [tokens, heads * head_dim]; out: bf16, the same shape (rows past the last sequence are left as they are)."""
+        cache, T, width = self.cache, batch.tokens, self.heads * self.cache.head_dim
+        _here(cache.device)
+        if batch.device != cache.device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {cache.device}")
+        ld_q, dt = _rows(q, T, width, "q", cache.device), _dtype(q, "q")
+        if out is None:
+            out = torch.empty((T, width), dtype=torch.bfloat16, device=q.device)
+        elif out.dtype != torch.bfloat16:
+            raise TypeError("out: bfloat16")
+        ld_o = _rows(out, T, width, "out", cache.device)
+        need = self._need.get(batch.max_new)
+        if need is None:
+            need = self._need[batch.max_new] = cache.lib.lx_b200_attention_workspace_bytes(cache.address, self.heads, batch.max_new)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        st = cache.lib.lx_b200_attention(cache.address, batch.address, q.data_ptr(), dt, ld_q, self.heads, self.scale, self.window, out.data_ptr(), ld_o,
+                                         ws.data_ptr() if need else None, _raw_stream())
+        if st:
+            raise RuntimeError(f"lx_b200_attention failed: {st}")
+        return out
+
+
+class NormResidual:
+    """The norm after a block (post), its gate, the scaled residual and the norm before the next block (pre), in one pass."""
+
+    def __init__(self, lib, width: int, pre: torch.Tensor | None = None, post: torch.Tensor | None = None, residual_scale: float = 1.0, block_scale: float = 1.0,
+                 gate_sigmoid: bool = False, eps: float = 1e-6):
+        self.lib, self.width, self.pre, self.post = lib, width, pre, post
+        self.residual_scale, self.block_scale, self.gate_sigmoid, self.eps = float(residual_scale), float(block_scale), int(gate_sigmoid), float(eps)
+        self._weight_dt = abi.BF16
+        for w, what in ((pre, "pre"), (post, "post")):
+            if w is not None:
+                if tuple(w.shape) != (width,) or not w.is_contiguous():
+                    raise ValueError(f"{what}: a contiguous vector of {width}")
+                self._weight_dt = _dtype(w, what)
+        if pre is not None and post is not None and (pre.dtype != post.dtype or pre.device != post.device):
+            raise ValueError("pre and post of one type on one device")
+
+    def __call__(self, y: torch.Tensor | None, h: torch.Tensor, gate: torch.Tensor | None = None, h_out: torch.Tensor | None = None,
+                 x: torch.Tensor | None = None):
+        """y: the block's output (None: nothing is added), h: the residual stream, both f32 or bf16 [T, width]; gate: [width] or [T, width].
+        Returns the new residual stream, in h's type (h_out may be h), and the next block's input (bf16 where x does not say
+        otherwise; None without a pre norm)."""
+        T, C = h.shape[0], self.width
+        _here(h.device)
+        ld_h, h_dt = _rows(h, T, C, "h"), _dtype(h, "h")
+        ld_y, y_dt = (0, abi.BF16) if y is None else (_rows(y, T, C, "y", h.device), _dtype(y, "y"))
+        ld_g, g_dt = 0, abi.BF16
+        if gate is not None:
+            g_dt = _dtype(gate, "gate")
+            if gate.dim() == 2:
+                ld_g = _rows(gate, T, C, "gate", h.device)
+            elif tuple(gate.shape) != (C,) or (C > 1 and gate.stride(0) != 1) or gate.device != h.device:
+                raise ValueError(f"gate: [{C}] or [{T}, {C}] on {h.device}")
+        for w in (self.pre, self.post):
+            if w is not None and w.device != h.device:
+                raise ValueError(f"the weights are on {w.device}, the rows on {h.device}")
+        if h_out is None:
+            h_out = torch.empty((T, C), dtype=h.dtype, device=h.device)
+        elif h_out.dtype != h.dtype:
+            raise TypeError("h_out of h's type")
+        ld_ho, ld_x, x_dt = _rows(h_out, T, C, "h_out", h.device), 0, abi.BF16
+        if self.pre is not None:
+            if x is None:
+                x = torch.empty((T, C), dtype=torch.bfloat16, device=h.device)
+            ld_x, x_dt = _rows(x, T, C, "x", h.device), _dtype(x, "x")
+        else:
+            x = None
+        st = self.lib.lx_b200_norm_residual(y.data_ptr() if y is not None else None, y_dt, ld_y, h.data_ptr(), h_dt, ld_h, gate.data_ptr() if gate is not None else None,
+                                            g_dt, ld_g, self.gate_sigmoid, self.post.data_ptr() if self.post is not None else None,
+                                            self.pre.data_ptr() if self.pre is not None else None, self._weight_dt, self.residual_scale, self.block_scale, self.eps,
+                                            h_out.data_ptr(), ld_ho, x.data_ptr() if x is not None else None, x_dt, ld_x, T, C, _raw_stream())
+        if st:
+            raise RuntimeError(f"lx_b200_norm_residual failed: {st}")
+        return h_out, x
+
+
+class AttentionBlock:
+    """An attention layer around one cache: the product of queries, keys and values, their append with the rotation on the way, attention,
+    the output product, and the norms, gate and residual that lead to the next block."""
+
+    def __init__(self, qkv: Linear, out: Linear, cache: KvCache, heads: int, norm: NormResidual, rotary: Rotary | None = None, scale: float | None = None,
+                 window: int = 0):
+        self.qkv, self.out, self.cache, self.heads, self.norm, self.rotary = qkv, out, cache, heads, norm, rotary
+        self.attention = Attention(cache, heads, scale=scale, window=window)
+        width, kv = heads * cache.head_dim, cache.kv_heads * cache.head_dim
+        if qkv.N != width + 2 * kv or out.K != width or out.N != norm.width:
+            raise ValueError("the products' sizes are not those of the heads and the norm")
+
+    def __call__(self, x: torch.Tensor, h: torch.Tensor, batch: KvBatch, positions: torch.Tensor | None = None, gate: torch.Tensor | None = None):
+        """x: the layer's input, normed, bf16 or f32 [tokens, K]; h: the residual stream. Returns what NormResidual returns."""
+        rows = self.qkv(x)
+        width, kv = self.heads * self.cache.head_dim, self.cache.kv_heads * self.cache.head_dim
+        q = self.cache.append(batch, rows[:, width:width + kv], rows[:, width + kv:], q=rows[:, :width], rotary=self.rotary, positions=positions)
+        return self.norm(self.out(self.attention(batch, q)), h, gate=gate)
+
+
 def expert_range(E: int, rank: int, world: int) -> tuple[int, int]:
     return E * rank // world, E * (rank + 1) // world
 

@@ -293,6 +293,65 @@ LX_API int64_t lx_b200_moe_static_scratch_bytes(void);
  * lx_b200_last_error() reads and clears it together with the library's own status word. */
 LX_API void* lx_b200_moe_static_scratch_ptr(void);
 
+/* ---- what an attention layer runs between its products (no counterpart in the ABI this library implements) ------------
+ *
+ * A paged cache of keys and values in 8 bits. Pages of page_tokens slots (16, 32, 64 or 128); k and v hold, page_stride
+ * bytes from one page to the next (a multiple of 16, the buffers on 16 bytes), codes [kv_heads][page_tokens][head_dim],
+ * E4M3 (LX_W_FP8) or signed bytes (LX_W_INT8); head_dim 64, 128 or 256. A value is code * scale, one f32 scale per page
+ * and head: k_scale, v_scale [pages][kv_heads]. A host struct of device pointers, like lx_weight. */
+typedef struct {
+  lx_wtype type;
+  int32_t kv_heads, head_dim, page_tokens;
+  int64_t pages, page_stride;
+  void *k, *v;
+  float *k_scale, *v_scale;
+} lx_b200_kv_cache;
+/* The sequences of a call (a host struct of device pointers). Sequence s owns the rows starts[s] .. starts[s + 1] - 1 of the
+ * call's row buffers, its new tokens (none is fine); lengths[s] counts its tokens in the cache with these; slot i of the
+ * sequence is slot i % page_tokens of page pages[s * ld_pages + i / page_tokens]. `tokens` rows are there in all: rows past
+ * starts[sequences] are left as they are. max_new: the most new tokens of one sequence, as far as the host knows; it chooses
+ * how the work is cut, a sequence with more is still computed. What the device arrays say is checked by the kernels: rows
+ * outside the buffers, a page outside the cache or a sequence shorter than its new tokens shows as 9 in lx_b200_last_error. */
+typedef struct {
+  int32_t sequences, tokens, max_new, ld_pages;
+  const int32_t *starts, *lengths, *pages;
+} lx_b200_kv_batch;
+/* Appends the new tokens' keys and values (rows of kv_heads * head_dim, f32 or bf16) to the cache; slots they had not reached are
+ * not touched. On the way the first rotary_dim values of every key head, and of every query head of q (q_heads of them; null: none),
+ * are turned by position * frequencies[j], j < rotary_dim / 2, in pairs (j, j + rotary_dim / 2), or (2 j, 2 j + 1) where
+ * `interleaved`: (a, b) -> (a cos - b sin, b cos + a sin). frequencies: f64, device; positions: one per row, null: the token's
+ * slot; rotary_dim a multiple of 8, 0: nothing turns. Turned queries go to q_out.
+ * A page's scale is the smallest power of two (2^-100 at least) that brings the largest magnitude of its tokens to 448 (INT8: 127)
+ * or less. It starts anew when the page's first slot is written; when a later token needs a larger one, the codes the page holds are
+ * rounded to it. Codes are rounded to nearest even. Values that are not finite make the page's scale of that head NaN, with codes
+ * of 0, until its first slot is written again: all of that page and head then reads as NaN. No two sequences of a call may write
+ * to one page. A sequence shorter than its new tokens, and tokens on a page outside the cache, are not written. */
+LX_API int lx_b200_kv_append(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* k, int ld_k, const void* v,
+                             int ld_v, lx_dtype kv_dtype, const void* q, lx_dtype q_dtype, int ld_q, int q_heads, void* q_out,
+                             lx_dtype q_out_dtype, int ld_q_out, const int32_t* positions, const double* frequencies, int rotary_dim,
+                             int interleaved, void* stream);
+/* Causal attention of the new tokens' queries over the cache (their own keys in it): query head h of the token in slot p reads
+ * head h / (q_heads / kv_heads) of the slots j <= p, with window > 0 of the last `window` of these (itself counted), and
+ * out = sum_j softmax_j(scale * q . k_j) v_j. q: rows of q_heads * head_dim, f32 or bf16; out the same in bf16; a query that sees no slot
+ * gets zeros. What unused slots and the table past a sequence's end hold is not read into any result; a page outside the
+ * cache makes the rows that see it NaN. f32 sums and statistics. workspace: lx_b200_attention_workspace_bytes, 16-byte aligned,
+ * what it holds does not matter; calls that may overlap need one each. A row's bits depend on the batch it is in (the keys of
+ * a sequence are cut to even out the work) and are the same every time. */
+LX_API int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q,
+                             int q_heads, float scale, int window, void* out, int ld_out, void* workspace, void* stream);
+/* For any batch with this cache's type and head_dim, these q_heads and this max_new; -1 for arguments the call refuses. */
+LX_API int64_t lx_b200_attention_workspace_bytes(const lx_b200_kv_cache* cache, int q_heads, int max_new);
+/* What follows a block and precedes the next, for T rows of C values:
+ *   u = y * rsqrt(mean(y^2) + eps) * post        (post null: u = y; y null: u = 0)
+ *   h_out = residual_scale * h + block_scale * gate * u      (gate null: 1; gate_sigmoid: 1 / (1 + exp(-gate)))
+ *   x = h_out * rsqrt(mean(h_out^2) + eps) * pre  (pre null: x is not written)
+ * gate: rows of C values, ld_gate apart (0: one row for all). h_out has h's type and may be h, or null: not written; x is
+ * computed from h_out before it is rounded. Sums in f32; a row's bits do not depend on T. */
+LX_API int lx_b200_norm_residual(const void* y, lx_dtype y_dtype, int ld_y, const void* h, lx_dtype h_dtype, int ld_h, const void* gate,
+                                 lx_dtype gate_dtype, int ld_gate, int gate_sigmoid, const void* post, const void* pre,
+                                 lx_dtype weight_dtype, float residual_scale, float block_scale, float eps, void* h_out, int ld_h_out,
+                                 void* x, lx_dtype x_dtype, int ld_x, int T, int C, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
