@@ -1,62 +1,479 @@
 // lx_b200_attention: causal attention of new tokens' queries over a paged 8-bit cache.
+//
+//   out = sum_j w_j v_j / sum_j w_j,   w_j = exp2(c q . k_j),   k_j = kscale kcode_j,  v_j = vscale vcode_j
+//
+// One pass over the keys. The 8-bit codes are exact in f16 and go to the tensor cores as they are; the scales stay outside, in f32:
+// t_j = c kscale (q . kcode_j) + log2 vscale, and with the running maximum m of these t the weights p_j = 2^(14 + t_j - m)
+// are what multiplies vcode_j, rounded to f16 (2^-11; below 2^-14 the step is 2^-24, which is 2^-38 of the largest weight), so pages of
+// very different loudness share one accumulator; the sum of the weights takes p_j 2^-14 / vscale, in f32.
 #include <algorithm>
 
-#include "kv.cuh"
+#include "attention.cuh"
 
 namespace b200 {
 namespace {
 
-struct AttentionArgs {
-  KvView kv;
-  const void* q;
-  uint16_t* out;
-  int64_t ld_q, ld_out;
-  int q_dtype, q_heads, group, window, int8;
-  float scale_log2;  // the softmax's scale times log2 e
-};
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kTile = 16 * kWarps;  // slots of a tile: 16 for each warp
 
-__device__ __forceinline__ float code_value(uint32_t code, int int8) {
-  return int8 ? static_cast<float>(static_cast<int8_t>(code)) : e4m3_to_f32(code);
+// Work of a sequence: units (blocks of ROWS query rows x key heads) of equally many tiles.
+struct SeqWork {
+  Span q;
+  int blocks, tile0, tiles;
+  int64_t all;
+  bool bad;
+};
+template <int ROWS>
+__device__ __forceinline__ SeqWork work_of(const AttentionArgs& A, int s) {
+  SeqWork w;
+  w.q = span_of(A.kv, s, w.bad);
+  w.blocks = (w.q.n * A.group + ROWS - 1) / ROWS;
+  const int first = w.q.length - w.q.n;
+  w.tile0 = A.window > 0 ? max(0, first - A.window + 1) / kTile : 0;
+  w.tiles = max(1, (w.q.length + kTile - 1) / kTile - w.tile0);
+  w.all = static_cast<int64_t>(w.blocks) * A.kv.kv_heads * w.tiles;
+  return w;
 }
 
-// One warp per query row and head: a running maximum and sum over the slots it sees, one slot after the other.
-template <int D>
-__global__ void __launch_bounds__(128) attention_rows_kernel(const __grid_constant__ AttentionArgs A) {
+// Every CTA has the same count of consecutive tiles of the whole batch, `per`; a unit that several CTAs share is joined by join_kernel.
+// Called by all threads; `sums`: shared. The sequence that holds tile `at` and its first tile's number come back in shared memory.
+struct Place {
+  int64_t total, base;  // base: tiles of the sequences before `seq`
+  int seq;              // -1: past the end
+};
+template <int ROWS>
+__device__ Place find_tile(const AttentionArgs& A, int64_t piece, int pieces, int64_t& per, int64_t& at, Place* shared, int64_t* sums) {
+  const int S = A.kv.sequences, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) shared->seq = -1;
+  int64_t total = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t base = 0;
+    for (int s0 = 0; s0 < S; s0 += kThreads) {
+      int64_t mine = 0;
+      if (s0 + tid < S) {
+        const SeqWork w = work_of<ROWS>(A, s0 + tid);
+        mine = w.all;
+        if (w.bad && piece == 0) report_batch(A.kv);
+      }
+      int64_t incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      __syncthreads();
+      if (lane == 31) sums[warp] = incl;
+      __syncthreads();
+      int64_t all = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) incl += sums[w];
+        all += sums[w];
+      }
+      const bool whole = S <= kThreads;  // one round: its sums serve both passes
+      if (pass == 0) total += all;
+      if (pass == 1 || whole) {
+        if (whole) {
+          per = max(static_cast<int64_t>(A.min_tiles), (total + pieces - 1) / pieces);
+          at = piece * per;
+        }
+        if (base + incl > at && base + incl - mine <= at) shared->seq = s0 + tid, shared->base = base + incl - mine;
+        base += all;
+        if (whole) pass = 1;
+        else if (base > at) break;
+      }
+    }
+    if (pass == 0) {
+      per = max(static_cast<int64_t>(A.min_tiles), (total + pieces - 1) / pieces);
+      at = piece * per;
+    }
+  }
+  __syncthreads();
+  return {total, shared->base, shared->seq};
+}
+
+// ---- codes to f16 pairs, exact ------------------------------------------------------------------------------------------
+template <bool kInt8>
+__device__ __forceinline__ void halves(uint32_t w, uint32_t& lo, uint32_t& hi) {  // codes 0, 1 and codes 2, 3
+  if constexpr (kInt8) {
+    const uint32_t u = w ^ 0x80808080u;  // code + 128, placed in the digits of 1024
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x), hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }" : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+template <int WORDS>
+__device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t (&w)[WORDS]) {
+  if constexpr (WORDS == 2) {
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4)
+      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "l"(p + 4 * i));
+  }
+}
+
+// What a warp needs of a step's page beside its codes.
+struct StepScale {
+  float k, log_v, inv_v;
+};
+__device__ __forceinline__ StepScale step_scale(const AttentionArgs& A, int page, int head) {
+  if (page < 0) {
+    const float nan = __uint_as_float(0x7fffffffu);
+    return {nan, nan, nan};
+  }
+  const int64_t at = static_cast<int64_t>(page) * A.kv.kv_heads + head;
+  const float v = A.kv.v_scale[at];
+  return {A.kv.k_scale[at], v, 0.0f};
+}
+
+// NT groups of 8 query rows against the keys of one head. D: values of a head.
+//
+// A warp takes 16 slots at a time. Both products have the keys as the 16-row operand and the query rows as the 8 columns, so that a
+// group of up to 8 queries wastes nothing: S^T = K Q^T, O^T += V^T P^T. The operands come straight from global memory into registers:
+// lane (g, t) loads a quarter row of keys g and g + 8 (which of a head's values share an instruction does not matter to a dot
+// product, the queries are laid out to match), and of values the dims g D/8 .. of slots 2t, 2t + 1, 2t + 8, 2t + 9, whose bytes are
+// interleaved before they are widened. P^T turns from accumulator to operand by one movmatrix per 8 x 8.
+template <bool kInt8, int D, int NT>
+__global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3 : 2) attention_stream_kernel(const __grid_constant__ AttentionArgs A) {
+  constexpr int ROWS = 8 * NT, KW = D / 16, VW = D / 32, MT = D / 16;
+  constexpr int OS = D + 4;  // row stride of the accumulators in shared memory
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint2* const qfrag = reinterpret_cast<uint2*>(smem);                     // [KW][NT][32]
+  float* const osum = reinterpret_cast<float*>(smem + KW * NT * 32 * 8);   // [kWarps][ROWS][OS]
+  float* const ms = osum + kWarps * ROWS * OS;                             // [kWarps][ROWS]
+  float* const ls = ms + kWarps * ROWS;                                    // [kWarps][ROWS]
+  float* const rowf = ls + kWarps * ROWS;                                  // [ROWS]
+  __shared__ Place place;
+  __shared__ int64_t sums[kWarps];
   pdl_wait();
   const KvView& C = A.kv;
-  const int lane = threadIdx.x & 31, h = blockIdx.y;
-  const int64_t row = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= C.tokens) return;
-  int s = -1, slot = 0;
-  for (int i = 0; i < C.sequences && s < 0; ++i) {
-    bool bad;
-    const Span q = span_of(C, i, bad);
-    if (bad && lane == 0) report_batch(C);
-    if (row >= q.row0 && row < q.row0 + q.n) s = i, slot = q.length - q.n + static_cast<int>(row) - q.row0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  int64_t per, at;
+  const Place start = find_tile<ROWS>(A, blockIdx.x, gridDim.x, per, at, &place, sums);
+  if (start.seq < 0) return;
+  const int64_t end = min(start.total, at + per);
+  int s = start.seq;
+  int64_t base = start.base;
+  const int log_p = __ffs(C.page_tokens) - 1, page_mask = C.page_tokens - 1;
+  while (at < end) {
+    const SeqWork W = work_of<ROWS>(A, s);
+    if (W.all == 0 || at >= base + W.all) {
+      base += W.all;
+      ++s;
+      continue;
+    }
+    // this CTA's part of one unit
+    const int unit = static_cast<int>((at - base) / W.tiles);
+    const int64_t unit_at = base + static_cast<int64_t>(unit) * W.tiles;
+    const int part0 = static_cast<int>(at - unit_at), part1 = static_cast<int>(min(static_cast<int64_t>(W.tiles), end - unit_at));
+    const int head = unit % C.kv_heads, row_block = unit / C.kv_heads * ROWS, rows = min(ROWS, W.q.n * A.group - row_block);
+    const int first = W.q.length - W.q.n;
+    // queries: each row times the power of two that brings it into f16's range
+    for (int r = warp; r < ROWS; r += kWarps) {
+      const int token = (row_block + r) / A.group, qh = head * A.group + (row_block + r) % A.group;
+      float v[(D + 127) / 128][4], most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < (D + 127) / 128; ++i) {
+        const int d = 4 * lane + 128 * i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = 0.0f;
+        if (r < rows && d < D) {
+          const int64_t src = (W.q.row0 + token) * A.ld_q + static_cast<int64_t>(qh) * D + d;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[i][j] = load_f32(A.q, A.q_dtype, src + j);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[i][j]));
+      }
+      const float up = f16_scale(warp_max(most));
+#pragma unroll
+      for (int i = 0; i < (D + 127) / 128; ++i) {
+        const int d = 4 * lane + 128 * i;
+        if (d >= D) continue;
+        const __half2 a = __floats2half2_rn(v[i][0] * up, v[i][1] * up), b = __floats2half2_rn(v[i][2] * up, v[i][3] * up);
+        qfrag[(d % (D / 4) / 4 * NT + r / 8) * 32 + r % 8 * 4 + d / (D / 4)] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      }
+      if (lane == 0) rowf[r] = A.scale_log2 / up;
+    }
+    __syncthreads();
+    // what lane (g, t) knows of its rows 8 nt + 2 t and + 1: the factor of their scores, the first slot past what they see
+    float f[NT][2];
+    int past[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * nt + 2 * t4 + e;
+        f[nt][e] = rowf[r];
+        past[nt][e] = r < rows ? first + (row_block + r) / A.group + 1 : 0;
+      }
+    const int past_low = first + row_block / A.group + 1, past_high = first + (row_block + rows - 1) / A.group + 1;  // of the first and the last row
+    const int see_low = A.window > 0 ? max(0, past_low - A.window) : 0;                                              // the first slot that any row sees
+    const int see_all = A.window > 0 ? max(0, past_high - A.window) : 0;                                             // from here on all rows do
+    float m[NT][2], l[NT][2], o[MT][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
+    }
+    // steps of 16 slots: this warp's every kWarps-th, those that some row sees
+    int step = (W.tile0 + part0) * kWarps + warp;
+    if (step < see_low / 16) step += (see_low / 16 - step + kWarps - 1) / kWarps * kWarps;
+    const int step_end = past_high <= 0 ? 0 : min((W.tile0 + part1) * kWarps, (past_high + 15) / 16);
+    uint32_t kw[2][KW], vw[4][VW];
+    auto page_at = [&](int st) {
+      if (st >= step_end) return 0;
+      const int p = page_of(C, s, st * 16 >> log_p);
+      if (p < 0 && lane == 0) report_batch(C);
+      return p;
+    };
+    auto slot_base = [&](int page, int st) {
+      return max(page, 0) * C.page_stride + (static_cast<int64_t>(head) * C.page_tokens + (st * 16 & page_mask)) * D;
+    };
+    auto load_k = [&](int64_t src) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) load_codes(C.k + src + (g + 8 * i) * D + t4 * (D / 4), kw[i]);
+    };
+    auto load_v = [&](int64_t src) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load_codes(C.v + src + (2 * t4 + (i & 1) + 8 * (i >> 1)) * D + g * (D / 8), vw[i]);
+    };
+    int page = page_at(step), page_next = page_at(step + kWarps);
+    StepScale sc{};
+    if (step < step_end) {
+      const int64_t src = slot_base(page, step);
+      load_k(src), load_v(src);
+      sc = step_scale(A, page, head);
+    }
+    for (; step < step_end; step += kWarps) {
+      const int slot = step * 16;
+      // scores
+      float x[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+        uint32_t a[4];
+        halves<kInt8>(kw[0][i], a[0], a[2]);
+        halves<kInt8>(kw[1][i], a[1], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint2 b = qfrag[(i * NT + nt) * 32 + lane];
+          mma16816<true>(x[nt], a, b.x, b.y);
+        }
+      }
+      // the next step's keys, and what it needs of its page
+      const bool more = step + kWarps < step_end;
+      const int64_t src_next = slot_base(page_next, step + kWarps);
+      const StepScale now = sc;
+      if (more) {
+        load_k(src_next);
+        sc = step_scale(A, page_next, head);
+      }
+      page = page_next;
+      page_next = page_at(step + 2 * kWarps);
+      const float v_scale = now.log_v < 0x1p-100f ? 0x1p-100f : now.log_v, log_v = __log2f(v_scale), inv_v = 0x1p-14f / v_scale;
+      const bool edge = slot + 16 > past_low || slot < see_all;
+      bool higher = false;
+      float shrink[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[nt][e] = fmaf(x[nt][e], f[nt][e & 1] * now.k, log_v);
+          if (edge) {
+            const int j = slot + g + 8 * (e >> 1), p = past[nt][e & 1];
+            if (j >= p || (A.window > 0 && j < p - A.window)) x[nt][e] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(x[nt][e], x[nt][e + 2]);
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
+          const float old = m[nt][e];
+          shrink[nt][e] = 1.0f;
+          if (top > old) {
+            m[nt][e] = top;
+            shrink[nt][e] = exp2_fast(old - top);
+            higher = true;
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          l[nt][0] *= shrink[nt][0], l[nt][1] *= shrink[nt][1];
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][nt][e] *= shrink[nt][e & 1];
+        }
+      }
+      uint32_t p0[NT], p1[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // a row that has seen nothing yet: 2^(-inf) and not 2^(-inf + inf)
+          p[e] = exp2_fast(x[nt][e] - (m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1] - 14.0f));
+        }
+        // a row that sees nothing of a page whose scale is not a number: nothing, and not 0 x NaN
+        if (const float w = p[0] + p[2]; w != 0.0f) l[nt][0] = fmaf(w, inv_v, l[nt][0]);
+        if (const float w = p[1] + p[3]; w != 0.0f) l[nt][1] = fmaf(w, inv_v, l[nt][1]);
+        const __half2 a = __floats2half2_rn(p[0], p[1]), b = __floats2half2_rn(p[2], p[3]);
+        p0[nt] = transpose8(*reinterpret_cast<const uint32_t*>(&a));
+        p1[nt] = transpose8(*reinterpret_cast<const uint32_t*>(&b));
+      }
+      if (slot + 16 > past_high || slot < see_low) {  // what no row sees may hold codes that are not numbers: 0 x NaN
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = slot + 2 * t4 + (i & 1) + 8 * (i >> 1);
+          if (j >= past_high || j < see_low)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vw[i][w] = 0;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t a[4];
+          halves<kInt8>(__byte_perm(vw[0][w], vw[1][w], half ? 0x7362 : 0x5140), a[0], a[1]);
+          halves<kInt8>(__byte_perm(vw[2][w], vw[3][w], half ? 0x7362 : 0x5140), a[2], a[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816<true>(o[2 * w + half][nt], a, p0[nt], p1[nt]);
+        }
+      }
+      if (more) load_v(src_next);
+    }
+    // the warps' parts meet in shared memory
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int sh = 4; sh < 32; sh <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], sh);
+        const int r = 8 * nt + 2 * t4 + e;
+        if (g == 0) ms[warp * ROWS + r] = m[nt][e], ls[warp * ROWS + r] = l[nt][e];
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+          *reinterpret_cast<float4*>(osum + (warp * ROWS + r) * OS + g * (D / 8) + 4 * w) =
+              make_float4(o[2 * w][nt][e], o[2 * w][nt][e + 2], o[2 * w + 1][nt][e], o[2 * w + 1][nt][e + 2]);
+      }
+    __syncthreads();
+    const bool complete = part0 == 0 && part1 == W.tiles;
+    const int64_t slot_ws = 2 * static_cast<int64_t>(blockIdx.x) + (part0 == 0);
+    for (int i = tid; i < rows * (D / 4); i += kThreads) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float top = ms[r], sum = 0.0f;
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, ms[w * ROWS + r]);
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = ms[w * ROWS + r], k = mw == -INFINITY ? 0.0f : exp2_fast(mw - top);
+        // a warp whose scores were all not-a-number has no maximum, its sums say so
+        const float lw = ls[w * ROWS + r];
+        sum += mw == -INFINITY ? lw : lw * k;
+        const float4 ow = *reinterpret_cast<const float4*>(osum + (w * ROWS + r) * OS + d);
+        v.x = fmaf(ow.x, k, v.x), v.y = fmaf(ow.y, k, v.y), v.z = fmaf(ow.z, k, v.z), v.w = fmaf(ow.w, k, v.w);
+      }
+      if (complete) {
+        const float inv = sum == 0.0f ? 0.0f : 0x1p-14f / sum;
+        const int token = (row_block + r) / A.group, qh = head * A.group + (row_block + r) % A.group;
+        store_out(A, (W.q.row0 + token) * A.ld_out + static_cast<int64_t>(qh) * D + d, v, inv);
+      } else {
+        float* dst = A.partial + slot_ws * (ROWS * (D + 2));
+        if (d == 0) dst[r] = top, dst[ROWS + r] = sum;
+        *reinterpret_cast<float4*>(dst + 2 * ROWS + r * D + d) = v;
+      }
+    }
+    __syncthreads();  // before the next unit's queries and sums
+    at = unit_at + part1;
   }
-  if (s < 0) return;
-  constexpr int V = D / 32;
-  float q[V], o[V] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < V; ++i) q[i] = load_f32(A.q, A.q_dtype, row * A.ld_q + h * D + lane * V + i) * A.scale_log2;
-  const int kvh = h / A.group, P = C.page_tokens;
-  for (int j = A.window > 0 ? max(0, slot - A.window + 1) : 0; j <= slot; ++j) {
-    const int page = page_of(C, s, j / P);
-    if (page < 0 && lane == 0) report_batch(C);
-    const int64_t at = max(page, 0) * C.page_stride + (static_cast<int64_t>(kvh) * P + j % P) * D + lane * V;
-    const int64_t sc = static_cast<int64_t>(max(page, 0)) * C.kv_heads + kvh;
-    float dot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) dot = fmaf(q[i], code_value(C.k[at + i], A.int8), dot);
-    dot = page < 0 ? __uint_as_float(0x7fffffffu) : warp_sum(dot) * C.k_scale[sc];
-    const float top = fmaxf(m, dot), shrink = m == -INFINITY ? 0.0f : exp2f(m - top), p = exp2f(dot - top), pv = p * C.v_scale[sc];
-    l = l * shrink + p;
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = fmaf(pv, code_value(C.v[at + i], A.int8), o[i] * shrink);
-    m = top;
+}
+
+// Joins the units that several CTAs of the stream kernel shared: CTA i the one that began in piece i and went on into the next.
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ AttentionArgs A) {
+  constexpr int ROWS = 8 * NT;
+  __shared__ Place place;
+  __shared__ int64_t sums[kWarps];
+  pdl_wait();
+  int64_t per, at;
+  const int pieces = gridDim.x;
+  const Place here = find_tile<ROWS>(A, blockIdx.x + 1, pieces, per, at, &place, sums);
+  if (here.seq < 0) return;
+  const SeqWork W = work_of<ROWS>(A, here.seq);
+  const int unit = static_cast<int>((at - here.base) / W.tiles);
+  const int64_t u0 = here.base + static_cast<int64_t>(unit) * W.tiles, u1 = u0 + W.tiles;
+  if (u0 == at || u0 < at - per) return;  // nothing crosses this border, or it began earlier
+  const int last = static_cast<int>((u1 - 1) / per);
+  const int head = unit % A.kv.kv_heads, row_block = unit / A.kv.kv_heads * ROWS, rows = min(ROWS, W.q.n * A.group - row_block);
+  const int64_t slot_floats = ROWS * (D + 2);
+  for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    float top = -INFINITY, sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = blockIdx.x; p <= last; ++p) {
+      const float* src = A.partial + (2 * static_cast<int64_t>(p) + (p == static_cast<int>(blockIdx.x))) * slot_floats;
+      const float mp = src[r], lp = src[ROWS + r], next = fmaxf(top, mp);
+      const float4 op = *reinterpret_cast<const float4*>(src + 2 * ROWS + r * D + d);
+      const float a = top == -INFINITY ? 0.0f : exp2_fast(top - next), b = mp == -INFINITY ? 0.0f : exp2_fast(mp - next);
+      sum = (top == -INFINITY ? sum : sum * a) + (mp == -INFINITY ? lp : lp * b);
+      v.x = v.x * a + op.x * b, v.y = v.y * a + op.y * b, v.z = v.z * a + op.z * b, v.w = v.w * a + op.w * b;
+      top = next;
+    }
+    const int token = (row_block + r) / A.group, qh = head * A.group + (row_block + r) % A.group;
+    store_out(A, (W.q.row0 + token) * A.ld_out + static_cast<int64_t>(qh) * D + d, v, sum == 0.0f ? 0.0f : 0x1p-14f / sum);
   }
-#pragma unroll
-  for (int i = 0; i < V; ++i) A.out[row * A.ld_out + h * D + lane * V + i] = static_cast<uint16_t>(f32_to_bf16_bits(slot < 0 ? 0.0f : o[i] / l));
+}
+
+template <int D, int NT>
+constexpr int stream_ctas() {
+  return NT * D <= 128 ? 4 : NT * D <= 256 ? 3 : 2;
+}
+template <int D, int NT>
+constexpr size_t stream_smem() {
+  return D / 16 * NT * 32 * 8 + sizeof(float) * (kWarps * 8 * NT * (D + 4) + 2 * kWarps * 8 * NT + 8 * NT);
+}
+template <int D, int NT>
+int64_t stream_workspace() {
+  return static_cast<int64_t>(sm_count()) * stream_ctas<D, NT>() * 2 * 8 * NT * (D + 2) * 4;
+}
+template <bool kInt8, int D, int NT>
+int launch_stream_attention(const AttentionArgs& A, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>(sm_count()) * stream_ctas<D, NT>();
+  if (grid == 0) return kNotSupported;
+  auto kernel = attention_stream_kernel<kInt8, D, NT>;
+  if (int e = allow_dynamic_smem<(kInt8 * 4 + (D == 64 ? 0 : D == 128 ? 1 : 2)) * 8 + NT>(kernel)) return e;
+  if (int e = launch_kernel(kernel, dim3(grid), dim3(kThreads), stream_smem<D, NT>(), stream, A)) return e;
+  return launch_kernel(attention_join_kernel<D, NT>, dim3(grid), dim3(kThreads), 0, stream, A);
+}
+// Groups of 8 rows that a CTA of the stream kernel takes at once: as few as hold a sequence's rows, 4 at most (2 with 256 values per
+// head), whose accumulators fill the registers.
+int row_groups(int head_dim, int64_t rows) { return rows <= 8 ? 1 : rows <= 16 || head_dim == 256 ? 2 : 4; }
+
+template <bool kInt8, int D>
+int stream_attention(const AttentionArgs& A, int64_t rows, cudaStream_t stream) {
+  const int nt = row_groups(D, rows);
+  if (nt == 1) return launch_stream_attention<kInt8, D, 1>(A, stream);
+  if (nt == 2) return launch_stream_attention<kInt8, D, 2>(A, stream);
+  if constexpr (D < 256) return launch_stream_attention<kInt8, D, 4>(A, stream);
+  return kNotSupported;
 }
 
 }  // namespace
@@ -66,7 +483,12 @@ using namespace b200;
 
 extern "C" int64_t lx_b200_attention_workspace_bytes(const lx_b200_kv_cache* cache, int q_heads, int max_new) {
   if (check_cache(cache) || q_heads < 1 || q_heads % cache->kv_heads || max_new < 0) return -1;
-  return 0;
+  const int nt = row_groups(cache->head_dim, static_cast<int64_t>(std::max(1, max_new)) * (q_heads / cache->kv_heads));
+  switch (cache->head_dim) {
+    case 64: return nt == 1 ? stream_workspace<64, 1>() : nt == 2 ? stream_workspace<64, 2>() : stream_workspace<64, 4>();
+    case 128: return nt == 1 ? stream_workspace<128, 1>() : nt == 2 ? stream_workspace<128, 2>() : stream_workspace<128, 4>();
+    default: return nt == 1 ? stream_workspace<256, 1>() : stream_workspace<256, 2>();
+  }
 }
 
 extern "C" int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q, int q_heads,
@@ -76,12 +498,21 @@ extern "C" int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv
   const int64_t width = static_cast<int64_t>(q_heads) * cache->head_dim;
   if (!valid_dtype(q_dtype) || q_heads < 1 || q_heads % cache->kv_heads || window < 0 || width > INT_MAX) return kInvalid;
   if (batch->sequences == 0 || batch->tokens == 0) return kOk;
-  if (!q || !out || ld_q < width || ld_out < width) return kInvalid;
+  if (static_cast<int64_t>(batch->tokens) * (q_heads / cache->kv_heads) > INT_MAX / 2) return kNotSupported;
+  if (!q || !out || ld_q < width || ld_out < width || !workspace || !aligned(workspace, 16)) return kInvalid;
   AttentionArgs A;
   A.kv = view_of(*cache, *batch);
-  A.q = q, A.out = static_cast<uint16_t*>(out), A.ld_q = ld_q, A.ld_out = ld_out;
-  A.q_dtype = q_dtype, A.q_heads = q_heads, A.group = q_heads / cache->kv_heads, A.window = window, A.int8 = cache->type == LX_W_INT8;
+  A.q = q, A.out = static_cast<uint16_t*>(out), A.ld_q = ld_q, A.ld_out = ld_out, A.partial = static_cast<float*>(workspace);
+  A.q_dtype = q_dtype, A.q_heads = q_heads, A.group = q_heads / cache->kv_heads, A.window = window;
+  A.out_vec = aligned(out, 8) && ld_out % 4 == 0;
   A.scale_log2 = scale * 1.4426950408889634f;
-  auto kernel = cache->head_dim == 64 ? attention_rows_kernel<64> : cache->head_dim == 128 ? attention_rows_kernel<128> : attention_rows_kernel<256>;
-  return launch_kernel(kernel, dim3((batch->tokens + 3) / 4, q_heads), dim3(128), 0, static_cast<cudaStream_t>(stream), A);
+  A.min_tiles = 2;
+  const int64_t rows = static_cast<int64_t>(std::max(1, batch->max_new)) * A.group;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool int8 = cache->type == LX_W_INT8;
+  switch (cache->head_dim) {
+    case 64: return int8 ? stream_attention<true, 64>(A, rows, st) : stream_attention<false, 64>(A, rows, st);
+    case 128: return int8 ? stream_attention<true, 128>(A, rows, st) : stream_attention<false, 128>(A, rows, st);
+    default: return int8 ? stream_attention<true, 256>(A, rows, st) : stream_attention<false, 256>(A, rows, st);
+  }
 }

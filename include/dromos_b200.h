@@ -297,8 +297,8 @@ LX_API void* lx_b200_moe_static_scratch_ptr(void);
  *
  * A paged cache of keys and values in 8 bits. Pages of page_tokens slots (16, 32, 64 or 128); k and v hold, page_stride
  * bytes from one page to the next (a multiple of 16, the buffers on 16 bytes), codes [kv_heads][page_tokens][head_dim],
- * E4M3 (LX_W_FP8) or signed bytes (LX_W_INT8); head_dim 64, 128 or 256. A value is code * scale, one f32 scale per page
- * and head: k_scale, v_scale [pages][kv_heads]. A host struct of device pointers, like lx_weight. */
+ * E4M3 (LX_W_FP8) or signed bytes (LX_W_INT8); head_dim 64, 128 or 256. A value is code * scale, one f32 scale, 0 or
+ * more, per page and head: k_scale, v_scale [pages][kv_heads]. A host struct of device pointers, like lx_weight. */
 typedef struct {
   lx_wtype type;
   int32_t kv_heads, head_dim, page_tokens;
