@@ -27,7 +27,8 @@ template <int ROWS>
 __device__ __forceinline__ SeqWork work_of(const AttentionArgs& A, int s) {
   SeqWork w;
   w.q = span_of(A.kv, s, w.bad);
-  w.blocks = (w.q.n * A.group + ROWS - 1) / ROWS;
+  const int rows = w.q.n * A.group;
+  w.blocks = rows <= A.most ? (rows + ROWS - 1) / ROWS : 0;
   const int first = w.q.length - w.q.n;
   w.tile0 = A.window > 0 ? max(0, first - A.window + 1) / kTile : 0;
   w.tiles = max(1, (w.q.length + kTile - 1) / kTile - w.tile0);
@@ -92,19 +93,6 @@ __device__ Place find_tile(const AttentionArgs& A, int64_t piece, int pieces, in
   return {total, shared->base, shared->seq};
 }
 
-// ---- codes to f16 pairs, exact ------------------------------------------------------------------------------------------
-template <bool kInt8>
-__device__ __forceinline__ void halves(uint32_t w, uint32_t& lo, uint32_t& hi) {  // codes 0, 1 and codes 2, 3
-  if constexpr (kInt8) {
-    const uint32_t u = w ^ 0x80808080u;  // code + 128, placed in the digits of 1024
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));
-    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
-    lo = *reinterpret_cast<const uint32_t*>(&x), hi = *reinterpret_cast<const uint32_t*>(&y);
-  } else {
-    asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }" : "=r"(lo), "=r"(hi) : "r"(w));
-  }
-}
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -481,14 +469,38 @@ int stream_attention(const AttentionArgs& A, int64_t rows, cudaStream_t stream) 
 
 using namespace b200;
 
-extern "C" int64_t lx_b200_attention_workspace_bytes(const lx_b200_kv_cache* cache, int q_heads, int max_new) {
-  if (check_cache(cache) || q_heads < 1 || q_heads % cache->kv_heads || max_new < 0) return -1;
-  const int nt = row_groups(cache->head_dim, static_cast<int64_t>(std::max(1, max_new)) * (q_heads / cache->kv_heads));
-  switch (cache->head_dim) {
+// Query rows per key head up to which a sequence goes to the stream kernel; more go to tiles of 128 rows (attention_tile.cu).
+static int stream_rows(int head_dim) { return head_dim == 256 ? 16 : 32; }
+
+static int64_t stream_workspace(int head_dim, int64_t rows) {
+  const int nt = row_groups(head_dim, rows);
+  switch (head_dim) {
     case 64: return nt == 1 ? stream_workspace<64, 1>() : nt == 2 ? stream_workspace<64, 2>() : stream_workspace<64, 4>();
     case 128: return nt == 1 ? stream_workspace<128, 1>() : nt == 2 ? stream_workspace<128, 2>() : stream_workspace<128, 4>();
     default: return nt == 1 ? stream_workspace<256, 1>() : stream_workspace<256, 2>();
   }
+}
+
+// Which kernels a call launches, and where their workspaces are.
+struct AttentionPlan {
+  bool tiles, streams;
+  int64_t rows;  // the most rows of a sequence that goes to the stream kernel
+  int64_t tiles_at, total;
+};
+static AttentionPlan attention_plan(const lx_b200_kv_cache& c, const lx_b200_kv_batch& b, int group) {
+  const int64_t rows = static_cast<int64_t>(std::max(1, b.max_new)) * group, limit = stream_rows(c.head_dim);
+  AttentionPlan p;
+  p.tiles = rows > limit, p.streams = !p.tiles || group <= limit;
+  // beside sequences of many new tokens, those of one are what the stream kernel is cut for
+  p.rows = p.tiles ? group : rows;
+  p.tiles_at = p.streams ? (stream_workspace(c.head_dim, p.rows) + 255) / 256 * 256 : 0;
+  p.total = p.tiles_at + (p.tiles ? tile_attention_workspace(c.head_dim, c.kv_heads, group, b.tokens, b.sequences) : 0);
+  return p;
+}
+
+extern "C" int64_t lx_b200_attention_workspace_bytes(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, int q_heads) {
+  if (check_cache(cache) || check_batch(batch) || q_heads < 1 || q_heads % cache->kv_heads) return -1;
+  return attention_plan(*cache, *batch, q_heads / cache->kv_heads).total;
 }
 
 extern "C" int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q, int q_heads,
@@ -507,12 +519,17 @@ extern "C" int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv
   A.out_vec = aligned(out, 8) && ld_out % 4 == 0;
   A.scale_log2 = scale * 1.4426950408889634f;
   A.min_tiles = 2;
-  const int64_t rows = static_cast<int64_t>(std::max(1, batch->max_new)) * A.group;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool int8 = cache->type == LX_W_INT8;
+  const AttentionPlan plan = attention_plan(*cache, *batch, A.group);
+  const int limit = stream_rows(cache->head_dim);
+  if (plan.tiles)
+    if (int e = tile_attention(A, cache->head_dim, int8, limit, static_cast<uint8_t*>(workspace) + plan.tiles_at, st)) return e;
+  if (!plan.streams) return kOk;
+  A.least = 1, A.most = plan.tiles ? limit : INT_MAX;
   switch (cache->head_dim) {
-    case 64: return int8 ? stream_attention<true, 64>(A, rows, st) : stream_attention<false, 64>(A, rows, st);
-    case 128: return int8 ? stream_attention<true, 128>(A, rows, st) : stream_attention<false, 128>(A, rows, st);
-    default: return int8 ? stream_attention<true, 256>(A, rows, st) : stream_attention<false, 256>(A, rows, st);
+    case 64: return int8 ? stream_attention<true, 64>(A, plan.rows, st) : stream_attention<false, 64>(A, plan.rows, st);
+    case 128: return int8 ? stream_attention<true, 128>(A, plan.rows, st) : stream_attention<false, 128>(A, plan.rows, st);
+    default: return int8 ? stream_attention<true, 256>(A, plan.rows, st) : stream_attention<false, 256>(A, plan.rows, st);
   }
 }

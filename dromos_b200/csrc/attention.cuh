@@ -5,7 +5,6 @@
 #include "tc.cuh"
 
 namespace b200 {
-namespace {
 
 struct AttentionArgs {
   KvView kv;
@@ -16,7 +15,10 @@ struct AttentionArgs {
   int q_dtype, q_heads, group, window, min_tiles;
   float scale_log2;  // the softmax's scale times log2 e
   bool out_vec;      // rows of `out` go on in pieces of four values
+  int least, most;   // the query rows per key head of the sequences that a kernel takes
 };
+
+namespace {
 
 // 2^x, 2^-22 relative, results below f32's normal range 0.
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -37,5 +39,24 @@ __device__ __forceinline__ void store_out(const AttentionArgs& A, int64_t at, co
   }
 }
 
+// ---- codes to f16 pairs, exact ------------------------------------------------------------------------------------------
+template <bool kInt8>
+__device__ __forceinline__ void halves(uint32_t w, uint32_t& lo, uint32_t& hi) {  // codes 0, 1 and codes 2, 3
+  if constexpr (kInt8) {
+    const uint32_t u = w ^ 0x80808080u;  // code + 128, placed in the digits of 1024
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x), hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }" : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+
 }  // namespace
+
+// attention_tile.cu: sequences of more than `limit` query rows per key head, in tiles of 128 rows on tcgen05. The workspace is its own.
+int64_t tile_attention_workspace(int head_dim, int kv_heads, int group, int tokens, int sequences);
+int tile_attention(AttentionArgs A, int head_dim, bool int8, int limit, void* workspace, cudaStream_t stream);
+
 }  // namespace b200

@@ -1,0 +1,805 @@
+// Attention of many query rows per key head (prompts, pieces of prompts, groups of drafted tokens): both products on tcgen05.
+//
+// The mathematics is that of attention.cu: codes widened exactly to f16, scales outside in f32, t_j = c kscale (q . kcode_j) + log2 vscale,
+// weights 2^(12 + t_j - m) that go to the second product in f16. m is a maximum the row had earlier: it moves when a larger one is more
+// than 3 above it (2^15 is inside f16's range), which spares the accumulator nearly every rescaling.
+//
+// A CTA takes 256 rows (128 where a head has 256 values) of one sequence and key head, a row being a new token and one of the heads that
+// share the keys, in two tiles of 128: S = Q K^T of one tile runs while the other's softmax does. Roles: two groups of four warps each
+// have a row per thread, hold its 128 scores in registers and write the weights back over them in tensor memory, as the first
+// operand of O += P V; one warp brings codes and scales in (bulk copies of 16 slots, so pages of any size); four warps widen keys and
+// values (values transposed: both operands of both products lie along the summed dimension, in core matrices of 8 x 16 bytes); one
+// thread issues the products. Values are stored with dim 4 l + j at n = 32 j + l, so that the four dims of a loaded word go to four
+// conflict-free stores; results are put back in order as they are read.
+//
+// The (row block, key head, key tile) triples of the batch are dealt evenly over the SMs in order, with kBlockCost tiles' worth of time
+// for beginning and ending a row block, so a CTA has part of at most two row blocks beside whole ones; parts are joined by a second
+// kernel. The order is laid out by a kernel of one CTA.
+#include <algorithm>
+
+#include "attention.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kRowTile = 128;
+constexpr int kSoftmaxWarps = 8, kWidenWarps = 4;
+constexpr int kMmaWarp = kSoftmaxWarps + kWidenWarps, kLoadWarp = kMmaWarp + 1;
+constexpr int kTileThreads = 32 * (kMmaWarp + 4);  // whole groups of four warps, each with its own share of the registers
+// Registers a thread: 128 at launch (512 threads), 65,536 in all; 256 x kSoftmaxRegs + 128 x kWidenRegs + 128 x kMmaRegs are as many.
+constexpr int kSoftmaxRegs = 192, kWidenRegs = 80, kMmaRegs = 48;
+static_assert(256 * kSoftmaxRegs + 128 * kWidenRegs + 128 * kMmaRegs <= 512 * 128, "more registers than the launch has");
+constexpr int kBlockCost = 3;
+constexpr int kShift = 12;  // the largest weights are 2^12 .. 2^15
+constexpr float kSlack = 3.0f, kUnshift = 0x1p-12f;
+
+template <int D>
+struct TileCfg {
+  static constexpr int kRowTiles = D == 256 ? 1 : 2;
+  static constexpr int kRows = kRowTiles * kRowTile;
+  static constexpr int kKeys = D == 256 ? 64 : 128;  // keys of a tile
+  static constexpr int kQBytes = kRowTile * D * 2, kKvBytes = kKeys * D * 2;
+  static constexpr int kRawBytes = kKeys * D;  // a tile's codes
+  static constexpr int kKOff = kRowTiles * kQBytes, kVOff = kKOff + 2 * kKvBytes, kRawOff = kVOff + 2 * kKvBytes, kScaleOff = kRawOff + 2 * kRawBytes;
+  static constexpr int kScaleGroups = kKeys / 16;
+  static constexpr int kBarOff = kScaleOff + 4 * kScaleGroups * 16;
+  static constexpr int kSmem = kBarOff + 256 < 120 * 1024 ? 120 * 1024 : kBarOff + 256;  // one CTA per SM: it takes all of tensor memory
+  static constexpr int kO = 256;  // first column of the accumulators of O; those of S begin at 0
+};
+
+struct BlockPlan {
+  int s, row_block, tile0, tiles;
+  int64_t before;  // the cost, in tiles, of the blocks before this one with all key heads
+};
+struct PlanHeader {
+  int64_t total;
+  int blocks;
+  int pad;
+};
+
+struct TileArgs {
+  AttentionArgs a;
+  PlanHeader* header;
+  BlockPlan* plan;
+  float* partial;
+  int capacity;  // blocks that `plan` has room for
+  bool q_vec, out_vec8;
+};
+
+// ---- the order of work -----------------------------------------------------------------------------------------------------
+template <int D>
+__global__ void __launch_bounds__(1024) attention_plan_kernel(const __grid_constant__ TileArgs T) {
+  using C = TileCfg<D>;
+  __shared__ int64_t sums[32];
+  pdl_wait();
+  const AttentionArgs& A = T.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto scan = [&](int64_t mine, int64_t& all) {  // the sum of the threads before
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    int64_t x = sums[lane], below = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+      const int64_t v = __shfl_sync(0xffffffffu, x, w);
+      if (w < warp) below += v;
+      all += v;
+    }
+    return below + incl - mine;
+  };
+  int64_t base = 0;
+  for (int s0 = 0; s0 < A.kv.sequences; s0 += 1024) {
+    int rows = 0;
+    Span q{};
+    if (s0 + tid < A.kv.sequences) {
+      bool bad;
+      q = span_of(A.kv, s0 + tid, bad);
+      rows = q.n * A.group;
+      if (bad) report_batch(A.kv);
+    }
+    const int blocks = rows >= A.least && rows <= A.most ? (rows + C::kRows - 1) / C::kRows : 0;
+    int64_t all;
+    const int64_t at = base + scan(blocks, all);
+    const int first = q.length - q.n;
+    for (int b = 0; b < blocks; ++b) {
+      if (at + b >= T.capacity) {  // sequences whose rows overlap: more blocks than there are rows
+        report_batch(A.kv);
+        break;
+      }
+      const int r0 = b * C::kRows, r1 = min(rows, r0 + C::kRows) - 1;
+      const int low = A.window > 0 ? max(0, first + r0 / A.group + 1 - A.window) : 0, past = max(0, first + r1 / A.group + 1);
+      const int tile0 = low / C::kKeys;
+      T.plan[at + b] = {s0 + tid, r0, tile0, max(1, (past + C::kKeys - 1) / C::kKeys - tile0), 0};
+    }
+    base += all;
+  }
+  const int count = static_cast<int>(min(base, static_cast<int64_t>(T.capacity)));
+  __syncthreads();
+  int64_t before = 0;
+  for (int b0 = 0; b0 < count; b0 += 1024) {
+    const int64_t mine = b0 + tid < count ? static_cast<int64_t>(T.plan[b0 + tid].tiles + kBlockCost) * A.kv.kv_heads : 0;
+    int64_t all;
+    const int64_t at = before + scan(mine, all);
+    if (b0 + tid < count) T.plan[b0 + tid].before = at;
+    before += all;
+  }
+  if (tid == 0) *T.header = {before, count, 0};
+}
+
+// A CTA's way through its share.
+struct Share {
+  int64_t at, end, per;
+  int block;
+};
+// The block that holds tile `at`; all threads of the CTA call it. found: shared.
+__device__ __forceinline__ int find_block(const TileArgs& T, int count, int64_t total, int64_t at, int* found) {
+  if (threadIdx.x == 0) *found = -1;
+  __syncthreads();
+  for (int b = threadIdx.x; b < count; b += blockDim.x) {
+    const int64_t lo = T.plan[b].before, hi = b + 1 < count ? T.plan[b + 1].before : total;
+    if (lo <= at && at < hi) *found = b;
+  }
+  __syncthreads();
+  return *found;
+}
+struct Part {
+  Span q;
+  int s, head, row_block, rows, tile, tiles;  // tile: the first one, of the sequence's slots
+  bool starts, whole;
+  int past_high, see_low;
+};
+template <int ROWS>
+__device__ __forceinline__ bool next_part(const TileArgs& T, Share& w, Part& p) {
+  const AttentionArgs& A = T.a;
+  const int heads = A.kv.kv_heads;
+  for (;;) {
+    if (w.at >= w.end) return false;
+    BlockPlan b = T.plan[w.block];
+    int cost = b.tiles + kBlockCost;
+    while (w.at >= b.before + static_cast<int64_t>(cost) * heads) b = T.plan[++w.block], cost = b.tiles + kBlockCost;
+    const int64_t in = w.at - b.before;
+    p.s = b.s, p.row_block = b.row_block, p.head = static_cast<int>(in / cost);
+    const int64_t u0 = b.before + static_cast<int64_t>(p.head) * cost;
+    const int c0 = static_cast<int>(w.at - u0), c1 = static_cast<int>(min(static_cast<int64_t>(cost), w.end - u0));
+    w.at = u0 + c1;
+    const int t0 = max(0, c0 - kBlockCost);
+    p.tiles = max(0, c1 - kBlockCost) - t0;
+    if (p.tiles == 0) continue;
+    p.tile = b.tile0 + t0;
+    p.starts = t0 == 0, p.whole = t0 == 0 && p.tiles == b.tiles;
+    bool bad;
+    p.q = span_of(A.kv, b.s, bad);
+    p.rows = min(ROWS, p.q.n * A.group - b.row_block);
+    const int first = p.q.length - p.q.n;
+    p.past_high = max(0, first + (b.row_block + p.rows - 1) / A.group + 1);
+    p.see_low = A.window > 0 ? max(0, first + b.row_block / A.group + 1 - A.window) : 0;
+    return true;
+  }
+}
+
+// ---- tensor memory and products -----------------------------------------------------------------------------------------------
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem descriptor], f16 operands; the descriptor in halves, as umma_ss_halves has them.
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p; .reg .b64 db; setp.ne.u32 p, %5, 0; mov.b64 db, {%2, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p; }" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// A warp's 32 query rows into their core matrices, each times the power of two that brings it into f16's range (and the sign of the
+// softmax's scale); lane r gets the factor of the scores of row r.
+template <int D, int DTYPE, bool VEC>
+__device__ __forceinline__ float load_queries(const AttentionArgs& A, const Part& p, int row, uint8_t* to, float sign) {
+  constexpr int V4 = (D + 127) / 128, BATCH = 8 / V4;
+  const int lane = threadIdx.x & 31;
+  float f = 0.0f;
+  int token = row / A.group, head = row % A.group;
+#pragma unroll 1
+  for (int j0 = 0; j0 < 32; j0 += BATCH) {
+    float4 x[BATCH][V4];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      // past the last row: its last row's values, so that no load waits for a condition; they are dropped below
+      const int64_t src = (p.q.row0 + min(token, p.q.n - 1)) * A.ld_q + (static_cast<int64_t>(p.head) * A.group + head) * D;
+#pragma unroll
+      for (int i = 0; i < V4; ++i) x[j][i] = load_row4(A.q, DTYPE < 0 ? A.q_dtype : DTYPE, src + (4 * lane + 128 * i) % D, VEC);
+      if (++head == A.group) head = 0, ++token;
+    }
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const bool there = row + j0 + j < p.row_block + p.rows;
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < V4; ++i) {
+        if (!there) x[j][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        most = fmaxf(fmaxf(fmaxf(most, fabsf(x[j][i].x)), fabsf(x[j][i].y)), fmaxf(fabsf(x[j][i].z), fabsf(x[j][i].w)));
+      }
+      const float up = f16_scale(warp_max(most)), by = up * sign;
+      if (lane == j0 + j) f = A.scale_log2 * sign / up;
+#pragma unroll
+      for (int i = 0; i < V4; ++i) {
+        const int d = 4 * lane + 128 * i;
+        const __half2 a = __floats2half2_rn(x[j][i].x * by, x[j][i].y * by), b = __floats2half2_rn(x[j][i].z * by, x[j][i].w * by);
+        if (d < D)
+          *reinterpret_cast<uint2*>(to + d / 8 * (kRowTile * 16) + (j0 + j) * 16 + d % 8 * 2) =
+              make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      }
+    }
+  }
+  return f;
+}
+
+// Eight results; whole: they lie on 16 bytes.
+__device__ __forceinline__ void store_out8(const AttentionArgs& A, int64_t at, const float4& a, const float4& b, float factor, bool whole) {
+  if (!whole) {
+    store_out(A, at, a, factor);
+    store_out(A, at + 4, b, factor);
+    return;
+  }
+  auto two = [&](float x, float y) { return f32_to_bf16_bits(x * factor) | f32_to_bf16_bits(y * factor) << 16; };
+  *reinterpret_cast<uint4*>(A.out + at) = make_uint4(two(a.x, a.y), two(a.z, a.w), two(b.x, b.y), two(b.z, b.w));
+}
+
+// ---- one row's softmax over a tile of scores -------------------------------------------------------------------------------------
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+// Two f32 at once.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// A row's scores of a tile, from tensor memory. EDGE: some row of the warps does not see all of it; this one sees the slots
+// lo <= j < hi of the tile.
+template <bool EDGE, int KT>
+__device__ __forceinline__ void mask_scores(uint32_t (&u)[KT / 32][32], int lo, int hi) {
+  if constexpr (EDGE) {
+#pragma unroll
+    for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (32 * c + j >= hi || 32 * c + j < lo) u[c][j] = 0xff800000u;
+  }
+}
+// The largest t of a tile.
+template <bool EDGE, int KT>
+__device__ __forceinline__ float tile_top(const uint32_t (&u)[KT / 32][32], const float4* sc, float f) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float a = __uint_as_float(u[c][16 * h]), b = __uint_as_float(u[c][16 * h + 1]);
+#pragma unroll
+      for (int j = 2; j < 14; j += 4) {
+        a = max3(a, __uint_as_float(u[c][16 * h + j]), __uint_as_float(u[c][16 * h + j + 1]));
+        b = max3(b, __uint_as_float(u[c][16 * h + j + 2]), __uint_as_float(u[c][16 * h + j + 3]));
+      }
+      const float most = fmaxf(max3(a, __uint_as_float(u[c][16 * h + 14]), __uint_as_float(u[c][16 * h + 15])), b);
+      const float4 g = sc[2 * c + h];
+      const float t = fmaf(most, f * g.x, g.y);
+      top = fmaxf(top, EDGE && most == -INFINITY ? -INFINITY : t);
+    }
+  return top;
+}
+// The weights of a tile, in f16 over its scores; returns what the sum of weights gains.
+template <bool EDGE, int KT>
+__device__ __forceinline__ float tile_weights(const uint32_t (&u)[KT / 32][32], uint32_t s_tmem, const float4* sc, float f, float from) {
+  float l = 0.0f;
+#pragma unroll
+  for (int c = 0; c < KT / 32; ++c) {
+    uint32_t w[16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 g = sc[2 * c + h];
+      const float by = f * g.x, add = g.y - from;
+      const uint64_t by2 = pack2(by, by), add_2 = pack2(add, add);
+      uint64_t sum2 = pack2(0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        const float u0 = __uint_as_float(u[c][16 * h + j]), u1 = __uint_as_float(u[c][16 * h + j + 1]);
+        float x0, x1;
+        unpack2(fma2(pack2(u0, u1), by2, add_2), x0, x1);
+        if constexpr (EDGE) {  // what a row does not see stays -inf, whatever the scale
+          x0 = u0 == -INFINITY ? u0 : x0;
+          x1 = u1 == -INFINITY ? u1 : x1;
+        }
+        x0 = exp2_fast(x0), x1 = exp2_fast(x1);
+        sum2 = add2(sum2, pack2(x0, x1));
+        const __half2 x = __floats2half2_rn(x0, x1);
+        w[8 * h + j / 2] = *reinterpret_cast<const uint32_t*>(&x);
+      }
+      float a, b;
+      unpack2(sum2, a, b);
+      // a row that sees nothing of a page whose scale is not a number: nothing, and not 0 x NaN
+      l = EDGE && a + b == 0.0f ? l : fmaf(a + b, g.z, l);
+    }
+    tmem_st16(s_tmem + 16 * c, w);
+  }
+  return l;
+}
+
+template <bool kInt8, int D>
+__global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const __grid_constant__ TileArgs T) {
+  using C = TileCfg<D>;
+  constexpr int RT = C::kRowTiles, KT = C::kKeys;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int found;
+  const AttentionArgs& A = T.a;
+  const KvView& V = A.kv;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t q_base = smem_u32(smem), k_base = q_base + C::kKOff, v_base = q_base + C::kVOff, raw_base = q_base + C::kRawOff, bars = q_base + C::kBarOff;
+  float4* const scales = reinterpret_cast<float4*>(smem + C::kScaleOff);  // [4][kScaleGroups]: kscale, log2 vscale, 2^-shift / vscale
+  const uint32_t q_full = bars, s_full = bars + 16, p_full = bars + 32, k_full = bars + 48, k_empty = bars + 64, v_full = bars + 80, v_empty = bars + 96,
+                 raw_full = bars + 112, raw_empty = bars + 128;  // raw: keys', values'
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + 8 * i, kRowTile);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, kRowTile);
+      mbar_init(k_full + 8 * i, 32 * kWidenWarps);
+      mbar_init(k_empty + 8 * i, 1);
+      mbar_init(v_full + 8 * i, 32 * kWidenWarps);
+      mbar_init(raw_full + 8 * i, 32);
+      mbar_init(raw_empty + 8 * i, 32 * kWidenWarps);
+      mbar_init(v_empty + 8 * i, 1);
+    }
+    mbar_init_fence();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&tmem_slot), kTmemColumns);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+  Share share;
+  {
+    const PlanHeader h = *T.header;
+    share.per = max(static_cast<int64_t>(A.min_tiles), (h.total + gridDim.x - 1) / gridDim.x);
+    share.at = blockIdx.x * share.per;
+    share.end = min(h.total, share.at + share.per);
+    share.block = find_block(T, h.blocks, h.total, share.at, &found);
+    if (share.block < 0) share.end = share.at;
+  }
+  Part p;
+  if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    // ================================ the products ================================
+    if (warp == kMmaWarp && lane == 0) {
+      const uint32_t idesc_s = (1u << 4) | (static_cast<uint32_t>(KT >> 3) << 17) | (static_cast<uint32_t>(kRowTile >> 4) << 24);
+      const uint32_t idesc_o = (1u << 4) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kRowTile >> 4) << 24);
+      // descriptors of core matrices (smem_desc): address and the step along the summed dimension, both in 16 bytes, below; the step of
+      // 128 bytes between groups of 8 rows above
+      const uint32_t desc_hi = (128u >> 4) | (1u << 14);
+      uint32_t kn = 0, vn = 0, qn[2] = {0, 0}, pn[2] = {0, 0};
+      bool ok = true;
+      auto scores = [&](int rt) {
+        const uint32_t qa = (q_base + rt * C::kQBytes) >> 4 | kRowTile << 16, kb = (k_base + (kn & 1) * C::kKvBytes) >> 4 | KT << 16;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          umma_ss_halves<kActF16>(tmem + rt * KT, qa + i * 2 * kRowTile, desc_hi, kb + i * 2 * KT, desc_hi, idesc_s, i > 0);
+      };
+      while (ok && next_part<C::kRows>(T, share, p)) {
+        const int tiles_of_rows = p.rows > kRowTile ? 2 : 1;
+        if (!tc_wait(k_full + 8 * (kn & 1), kn >> 1 & 1, V.status)) break;
+        for (int rt = 0; rt < tiles_of_rows && ok; ++rt) {
+          ok = tc_wait(q_full + 8 * rt, qn[rt]++ & 1, V.status);
+          if (!ok) break;
+          tc_fence_after();
+          scores(rt);
+          umma_commit(s_full + 8 * rt);
+        }
+        if (!ok) break;
+        umma_commit(k_empty + 8 * (kn & 1));
+        ++kn;
+        for (int i = 0; i < p.tiles && ok; ++i) {
+          const bool more = i + 1 < p.tiles;
+          for (int rt = 0; rt < tiles_of_rows; ++rt) {
+            if ((rt == 0 && !tc_wait(v_full + 8 * (vn & 1), vn >> 1 & 1, V.status)) || !tc_wait(p_full + 8 * rt, pn[rt] & 1, V.status) ||
+                (rt == 0 && more && !tc_wait(k_full + 8 * (kn & 1), kn >> 1 & 1, V.status))) {
+              ok = false;
+              break;
+            }
+            ++pn[rt];
+            tc_fence_after();
+            const uint32_t vb = (v_base + (vn & 1) * C::kKvBytes) >> 4 | D << 16;
+#pragma unroll
+            for (int j = 0; j < KT / 16; ++j)
+              umma_ts(tmem + C::kO + rt * D, tmem + rt * KT + 8 * j, vb + j * 2 * D, desc_hi, idesc_o, i > 0 || j > 0);
+            if (more) scores(rt);
+            umma_commit(s_full + 8 * rt);  // the next scores, or, after the last tile, the sums
+          }
+          if (!ok) break;
+          umma_commit(v_empty + 8 * (vn & 1));
+          ++vn;
+          if (more) {
+            umma_commit(k_empty + 8 * (kn & 1));
+            ++kn;
+          }
+        }
+      }
+    }
+    else if (warp == kLoadWarp) {
+      // codes and scales: lane g has the slots 16 g .. 16 g + 15 of a tile
+      const int log_p = __ffs(V.page_tokens) - 1, page_mask = V.page_tokens - 1;
+      uint32_t n = 0, sent[2] = {0, 0};
+      bool ok = true;
+      while (ok && next_part<C::kRows>(T, share, p)) {
+        for (int i = 0; i < p.tiles && ok; ++i, ++n) {
+          const int slot = (p.tile + i) * KT + 16 * lane;
+          int page = -2;  // nothing that any row sees
+          if (lane < C::kScaleGroups && slot < p.past_high && slot + 16 > p.see_low) {
+            page = page_of(V, p.s, slot >> log_p);
+            if (page < 0) report_batch(V);
+          }
+          const int64_t src = max(page, 0) * V.page_stride + (static_cast<int64_t>(p.head) * V.page_tokens + (slot & page_mask)) * D;
+          if (lane < C::kScaleGroups) {
+            const float nan = __uint_as_float(0x7fffffffu);
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // the last one: whether there are codes
+            if (page == -1) s = make_float4(nan, nan, nan, 0.0f);
+            if (page >= 0) {
+              const int64_t at = static_cast<int64_t>(page) * V.kv_heads + p.head;
+              const float v = V.v_scale[at], vs = v < 0x1p-100f ? 0x1p-100f : v;
+              s = make_float4(V.k_scale[at], __log2f(vs), kUnshift / vs, 1.0f);
+            }
+            scales[(n & 3) * C::kScaleGroups + lane] = s;
+          }
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            ok = tc_wait(raw_empty + 8 * kv, (n & 1) ^ 1, V.status);
+            if (!ok) break;
+            const uint32_t bar = raw_full + 8 * kv;
+            if (page >= 0) {
+              mbar_arrive_expect_tx(bar, 16 * D);
+              bulk_g2s(raw_base + kv * C::kRawBytes + 16 * lane * D, (kv ? V.v : V.k) + src, 16 * D, bar);
+            } else {
+              mbar_arrive(bar);
+            }
+            ++sent[kv];
+          }
+        }
+      }
+      // copies in flight end before the CTA does
+      for (int kv = 0; kv < 2; ++kv)
+        if (sent[kv] > 0) tc_wait(raw_full + 8 * kv, (sent[kv] - 1) & 1, V.status);
+    }
+  } else if (warp < kSoftmaxWarps) {
+    // ================================ softmax: a row per thread ================================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int rt = warp >> 2, row = tid & (kRowTile - 1);
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t s_tmem = tmem + lanes + rt * KT, o_tmem = tmem + lanes + C::kO + rt * D;
+    uint32_t sn = 0, tiles_done = 0;
+    bool ok = true;
+    const float sign = A.scale_log2 < 0.0f ? -1.0f : 1.0f;
+    while (ok && next_part<C::kRows>(T, share, p)) {
+      const int first = p.q.length - p.q.n, row0 = p.row_block + rt * kRowTile;
+      const bool mine = rt < RT && (rt == 0 || p.rows > kRowTile);
+      float f = 0.0f;
+      if (mine) {
+        // the rows of this warp's lanes, each times the power of two that brings it into f16's range
+        const int w_row = 32 * (warp & 3);
+        if (T.q_vec && A.q_dtype == LX_BF16) f = load_queries<D, LX_BF16, true>(A, p, row0 + w_row, smem + rt * C::kQBytes + w_row * 16, sign);
+        else if (T.q_vec) f = load_queries<D, LX_F32, true>(A, p, row0 + w_row, smem + rt * C::kQBytes + w_row * 16, sign);
+        else f = load_queries<D, -1, false>(A, p, row0 + w_row, smem + rt * C::kQBytes + w_row * 16, sign);
+        proxy_fence();
+        mbar_arrive(q_full + 8 * rt);
+      }
+      if (!mine) {
+        tiles_done += p.tiles;
+        continue;
+      }
+      const int r = row0 + row;
+      const bool valid = r < p.row_block + p.rows;
+      const int past = valid ? first + r / A.group + 1 : 0;
+      const int past_low = first + row0 / A.group + 1, past_last = first + (min(row0 + kRowTile, p.row_block + p.rows) - 1) / A.group + 1;
+      const int see_all = A.window > 0 ? past_last - A.window : 0, low = A.window > 0 ? past - A.window : 0;
+      float m = -INFINITY, l = 0.0f;
+      for (int i = 0; i < p.tiles; ++i) {
+        const int key0 = (p.tile + i) * KT;
+        const float4* sc = scales + ((tiles_done + i) & 3) * C::kScaleGroups;
+        if (!tc_wait(s_full + 8 * rt, sn & 1, V.status)) {
+          ok = false;
+          break;
+        }
+        ++sn;
+        __syncwarp();
+        tc_fence_after();
+        const bool edge = key0 + KT > past_low || key0 < see_all;
+        const int lo = low - key0, hi = past - key0;
+        uint32_t u[KT / 32][32];
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) tmem_ld32(s_tmem + 32 * c, u[c]);
+        tmem_wait_ld();
+        float top;
+        if (edge) {
+          mask_scores<true, KT>(u, lo, hi);
+          top = tile_top<true, KT>(u, sc, f);
+        } else {
+          top = tile_top<false, KT>(u, sc, f);
+        }
+        const bool higher = top > m + kSlack;  // at first m is -inf
+        if (__any_sync(0xffffffffu, higher)) {
+          const float shrink = higher ? exp2_fast(m - top) : 1.0f;
+          m = higher ? top : m;
+          if (i > 0) {
+            l *= shrink;
+            // the scores of this tile came after the product of the tile before: nothing is at work on these sums
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t v[16];
+              tmem_ld16(o_tmem + 16 * c, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * shrink);
+              tmem_st16(o_tmem + 16 * c, v);
+            }
+          }
+        }
+        const float from = (m == -INFINITY ? 0.0f : m) - kShift;
+        l += edge ? tile_weights<true, KT>(u, s_tmem, sc, f, from) : tile_weights<false, KT>(u, s_tmem, sc, f, from);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_full + 8 * rt);
+      }
+      tiles_done += p.tiles;
+      if (!ok || !tc_wait(s_full + 8 * rt, sn & 1, V.status)) {
+        ok = false;
+        break;
+      }
+      ++sn;
+      __syncwarp();
+      tc_fence_after();
+      float* const part = T.partial + (2 * static_cast<int64_t>(blockIdx.x) + p.starts) * (C::kRows * (D + 2));
+      const int pr = rt * kRowTile + row;
+      const int64_t out_row = (p.q.row0 + r / A.group) * A.ld_out + (static_cast<int64_t>(p.head) * A.group + r % A.group) * D;
+      const float factor = l == 0.0f ? 0.0f : kUnshift / l;
+      if (!p.whole && valid) part[pr] = m, part[C::kRows + pr] = l;
+      constexpr int W = D < 128 ? D / 4 : 32;  // dim 4 l + j of a run of 4 W lies at n = W j + l
+#pragma unroll
+      for (int h = 0; h < D / (4 * W); ++h)
+#pragma unroll
+        for (int k = 0; k < W / 16; ++k) {
+          uint32_t u[4][16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tmem_ld16(o_tmem + 4 * W * h + W * j + 16 * k, u[j]);
+          tmem_wait_ld();
+          if (valid) {
+#pragma unroll
+            for (int q = 0; q < 16; q += 2) {
+              const int d = 4 * (W * h + 16 * k + q);
+              const float4 a = make_float4(__uint_as_float(u[0][q]), __uint_as_float(u[1][q]), __uint_as_float(u[2][q]), __uint_as_float(u[3][q]));
+              const float4 b = make_float4(__uint_as_float(u[0][q + 1]), __uint_as_float(u[1][q + 1]), __uint_as_float(u[2][q + 1]), __uint_as_float(u[3][q + 1]));
+              if (p.whole) {
+                store_out8(A, out_row + d, a, b, factor, T.out_vec8);
+              } else {
+                *reinterpret_cast<float4*>(part + 2 * C::kRows + pr * D + d) = a;
+                *reinterpret_cast<float4*>(part + 2 * C::kRows + pr * D + d + 4) = b;
+              }
+            }
+          }
+          __syncwarp();
+        }
+      tc_fence_before();  // the next block's products come after this thread's next arrival
+    }
+  } else {
+    // ================================ keys and values, widened ================================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs));
+    const int w4 = warp & 3;
+    constexpr int WK = KT / 4;  // slots of a tile that one warp has
+    const uint8_t* const raw_k = smem + C::kRawOff;
+    const uint8_t* const raw_v = raw_k + C::kRawBytes;
+    uint32_t n = 0;
+    bool ok = true;
+    while (ok && next_part<C::kRows>(T, share, p)) {
+      for (int i = 0; i < p.tiles && ok; ++i, ++n) {
+        const int slot0 = (p.tile + i) * KT;
+        const bool all = slot0 >= p.see_low && slot0 + KT <= p.past_high;  // else what no row sees, which was not copied, reads as 0
+        auto seen = [&](int j) { return all || (slot0 + j < p.past_high && slot0 + j >= p.see_low); };
+        // keys. Lane i of eight takes key i of a run, and of its pieces of 16 bytes another one than its neighbours: neither the reads of
+        // rows nor the writes of core matrices meet in a bank
+        if (!tc_wait(raw_full, n & 1, V.status) || !tc_wait(k_empty + 8 * (n & 1), (n >> 1 & 1) ^ 1, V.status)) {
+          ok = false;
+          break;
+        }
+        {
+          constexpr int PIECES = D / 16;
+          const uint32_t dst = k_base + (n & 1) * C::kKvBytes;
+          const int key8 = lane & 7;
+#pragma unroll
+          for (int a = 0; a < WK / 8; ++a) {
+            const int key = w4 * WK + 8 * a + key8;
+            const bool use = seen(key) && scales[(n & 3) * C::kScaleGroups + key / 16].w != 0.0f;
+#pragma unroll
+            for (int b = 0; b < PIECES / 4; ++b) {
+              const int piece = ((D == 64 ? key8 >> 1 : key8) + 4 * b + (lane >> 3)) & (PIECES - 1);
+              uint4 x = *reinterpret_cast<const uint4*>(raw_k + key * D + 16 * piece);
+              if (!use) x = make_uint4(0, 0, 0, 0);
+              const uint32_t word[4] = {x.x, x.y, x.z, x.w};
+              uint32_t o[8];
+#pragma unroll
+              for (int c = 0; c < 4; ++c) halves<kInt8>(word[c], o[2 * c], o[2 * c + 1]);
+              const uint32_t to = dst + 2 * piece * (KT * 16) + key * 16;
+              sts128(to, o[0], o[1], o[2], o[3]);
+              sts128(to + KT * 16, o[4], o[5], o[6], o[7]);
+            }
+          }
+        }
+        mbar_arrive(raw_empty);
+        proxy_fence();
+        mbar_arrive(k_full + 8 * (n & 1));
+        // values: lane: four dims of eight keys; with 64 values per head the half warps have a run of eight keys each
+        if (!tc_wait(raw_full + 8, n & 1, V.status) || !tc_wait(v_empty + 8 * (n & 1), (n >> 1 & 1) ^ 1, V.status)) {
+          ok = false;
+          break;
+        }
+        {
+          constexpr int LANES = D < 128 ? D / 4 : 32, AT_ONCE = 32 / LANES, RUNS = WK / (8 * AT_ONCE), HALVES = D > 128 ? 2 : 1;
+          const int l = lane % LANES, sub = lane / LANES;
+          const uint32_t dst = v_base + (n & 1) * C::kKvBytes;
+#pragma unroll
+          for (int a = 0; a < RUNS; ++a) {
+            const int run = w4 * (WK / 8) + a * AT_ONCE + sub;
+            const bool use = scales[(n & 3) * C::kScaleGroups + run / 2].w != 0.0f;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) {
+              uint32_t x[8], o[4][4];  // o: dim, pair of keys
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                x[j] = *reinterpret_cast<const uint32_t*>(raw_v + (8 * run + j) * D + 128 * h + 4 * l);
+                if (!use || !seen(8 * run + j)) x[j] = 0;
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                halves<kInt8>(__byte_perm(x[2 * j], x[2 * j + 1], 0x5140), o[0][j], o[1][j]);
+                halves<kInt8>(__byte_perm(x[2 * j], x[2 * j + 1], 0x7362), o[2][j], o[3][j]);
+              }
+              const uint32_t to = dst + run * (D * 16) + (128 * h + l) * 16;
+#pragma unroll
+              for (int d = 0; d < 4; ++d) sts128(to + d * LANES * 16, o[d][0], o[d][1], o[d][2], o[d][3]);
+            }
+          }
+        }
+        mbar_arrive(raw_empty + 8);
+        proxy_fence();
+        mbar_arrive(v_full + 8 * (n & 1));
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemColumns);
+}
+
+// Joins the row blocks that several CTAs shared: CTA (i, j) rows of the one that began in share i and went on into the next.
+template <int D>
+__global__ void __launch_bounds__(256) attention_tile_join_kernel(const __grid_constant__ TileArgs T, int shares) {
+  using C = TileCfg<D>;
+  __shared__ int found;
+  pdl_wait();
+  const AttentionArgs& A = T.a;
+  const PlanHeader h = *T.header;
+  const int64_t per = max(static_cast<int64_t>(A.min_tiles), (h.total + shares - 1) / shares), at = (blockIdx.x + 1) * per;
+  const int block = find_block(T, h.blocks, h.total, at, &found);
+  if (block < 0) return;
+  const BlockPlan b = T.plan[block];
+  const int cost = b.tiles + kBlockCost, head = static_cast<int>((at - b.before) / cost);
+  const int64_t u1 = b.before + static_cast<int64_t>(head + 1) * cost, first_tile = u1 - b.tiles;
+  if (first_tile >= at || first_tile < at - per) return;  // nothing crosses this border, or it began earlier
+  const int last = static_cast<int>((u1 - 1) / per);
+  bool bad;
+  const Span q = span_of(A.kv, b.s, bad);
+  const int rows = min(C::kRows, q.n * A.group - b.row_block);
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * (D / 4); i += gridDim.y * 256) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    float top = -INFINITY, sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = blockIdx.x; p <= last; ++p) {
+      const float* src = T.partial + (2 * static_cast<int64_t>(p) + (p == static_cast<int>(blockIdx.x))) * (C::kRows * (D + 2));
+      const float mp = src[r], lp = src[C::kRows + r], next = fmaxf(top, mp);
+      const float4 op = *reinterpret_cast<const float4*>(src + 2 * C::kRows + r * D + d);
+      const float x = top == -INFINITY ? 0.0f : exp2_fast(top - next), y = mp == -INFINITY ? 0.0f : exp2_fast(mp - next);
+      sum = (top == -INFINITY ? sum : sum * x) + (mp == -INFINITY ? lp : lp * y);
+      v.x = v.x * x + op.x * y, v.y = v.y * x + op.y * y, v.z = v.z * x + op.z * y, v.w = v.w * x + op.w * y;
+      top = next;
+    }
+    const int rr = b.row_block + r;
+    store_out(A, (q.row0 + rr / A.group) * A.ld_out + (static_cast<int64_t>(head) * A.group + rr % A.group) * D + d, v, sum == 0.0f ? 0.0f : kUnshift / sum);
+  }
+}
+
+struct TileLayout {
+  int64_t plan, partial, total;
+  int capacity;
+};
+TileLayout tile_layout(int head_dim, int kv_heads, int group, int tokens, int sequences) {
+  const int rows = head_dim == 256 ? kRowTile : 2 * kRowTile;
+  TileLayout L;
+  // a block holds more than 0 rows: whole blocks of all rows, and a last one of each sequence
+  L.capacity = static_cast<int>(static_cast<int64_t>(tokens) * group / rows + sequences);
+  L.plan = 64;
+  L.partial = (L.plan + static_cast<int64_t>(L.capacity) * static_cast<int64_t>(sizeof(BlockPlan)) + 255) / 256 * 256;
+  L.total = L.partial + static_cast<int64_t>(sm_count()) * 2 * rows * (head_dim + 2) * 4;
+  return L;
+}
+
+template <bool kInt8, int D>
+int launch_tile(const TileArgs& T, cudaStream_t stream) {
+  using C = TileCfg<D>;
+  const unsigned grid = static_cast<unsigned>(sm_count());
+  if (grid == 0) return kNotSupported;
+  auto kernel = attention_tile_kernel<kInt8, D>;
+  if (int e = allow_big_smem<kInt8 * 4 + (D == 64 ? 0 : D == 128 ? 1 : 2)>(kernel)) return e;
+  if (int e = launch_kernel(attention_plan_kernel<D>, dim3(1), dim3(1024), 0, stream, T)) return e;
+  if (int e = launch_kernel(kernel, dim3(grid), dim3(kTileThreads), C::kSmem, stream, T)) return e;
+  return launch_kernel(attention_tile_join_kernel<D>, dim3(grid, 8), dim3(256), 0, stream, T, static_cast<int>(grid));
+}
+
+}  // namespace
+
+int64_t tile_attention_workspace(int head_dim, int kv_heads, int group, int tokens, int sequences) {
+  return tile_layout(head_dim, kv_heads, group, tokens, sequences).total;
+}
+
+int tile_attention(AttentionArgs A, int head_dim, bool int8, int limit, void* workspace, cudaStream_t stream) {
+  const TileLayout L = tile_layout(head_dim, A.kv.kv_heads, A.group, A.kv.tokens, A.kv.sequences);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  TileArgs T;
+  T.a = A;
+  T.a.least = limit + 1, T.a.most = INT_MAX;
+  T.a.min_tiles = 2 * kBlockCost + 2;
+  T.header = reinterpret_cast<PlanHeader*>(ws), T.plan = reinterpret_cast<BlockPlan*>(ws + L.plan), T.partial = reinterpret_cast<float*>(ws + L.partial);
+  T.capacity = L.capacity;
+  T.out_vec8 = aligned(A.out, 16) && A.ld_out % 8 == 0;
+  T.q_vec = aligned(A.q, A.q_dtype == LX_BF16 ? 8 : 16) && A.ld_q % 4 == 0;
+  switch (head_dim) {
+    case 64: return int8 ? launch_tile<true, 64>(T, stream) : launch_tile<false, 64>(T, stream);
+    case 128: return int8 ? launch_tile<true, 128>(T, stream) : launch_tile<false, 128>(T, stream);
+    default: return int8 ? launch_tile<true, 256>(T, stream) : launch_tile<false, 256>(T, stream);
+  }
+}
+
+}  // namespace b200

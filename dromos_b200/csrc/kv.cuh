@@ -6,11 +6,6 @@
 #include "launch.cuh"
 
 namespace b200 {
-namespace {
-
-// Smallest and largest exponent of a scale the append writes. The lower end keeps the sum of a softmax's weights, which are
-// held divided by these scales, inside f32: 2^100 times a million tokens is 2^120. No f32 needs one above the upper end.
-constexpr int kScaleMin = -100, kScaleMax = 122;
 
 struct KvView {
   uint8_t *k, *v;
@@ -21,6 +16,12 @@ struct KvView {
   int sequences, tokens, ld_pages;
   int* status;
 };
+
+namespace {
+
+// Smallest and largest exponent of a scale the append writes. The lower end keeps the sum of a softmax's weights, which are
+// held divided by these scales, inside f32: 2^100 times a million tokens is 2^120. No f32 needs one above the upper end.
+constexpr int kScaleMin = -100, kScaleMax = 122;
 
 // A sequence's rows and slots, 0 new tokens where what the arrays say cannot be.
 struct Span {
@@ -39,6 +40,16 @@ __device__ __forceinline__ int page_of(const KvView& A, int s, int i) {
 }
 __device__ __forceinline__ void report_batch(const KvView& A) {
   if (A.status) atomicExch(A.status, kStatusBatch);
+}
+
+// Four values of a row; vec: they lie on a boundary of their size.
+__device__ __forceinline__ float4 load_row4(const void* p, int dtype, int64_t i, bool vec) {
+  if (vec) {
+    if (dtype == LX_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+  }
+  return make_float4(load_f32(p, dtype, i), load_f32(p, dtype, i + 1), load_f32(p, dtype, i + 2), load_f32(p, dtype, i + 3));
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------

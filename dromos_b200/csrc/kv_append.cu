@@ -24,14 +24,6 @@ struct AppendArgs {
   const double* frequencies;
 };
 
-__device__ __forceinline__ float4 load4(const void* p, int dtype, int64_t i, bool vec) {
-  if (vec) {
-    if (dtype == LX_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-  }
-  return make_float4(load_f32(p, dtype, i), load_f32(p, dtype, i + 1), load_f32(p, dtype, i + 2), load_f32(p, dtype, i + 3));
-}
 __device__ __forceinline__ void store4(void* p, int dtype, int64_t i, const float* v, bool vec) {
   if (!vec) {
 #pragma unroll
@@ -55,7 +47,7 @@ __device__ __forceinline__ Piece piece_of(const AppendArgs& A, int u) {
 }
 // The eight values of a piece, turned by the angles at cs.
 __device__ __forceinline__ void load_piece(const AppendArgs& A, const void* p, int dtype, int64_t head, const Piece& u, bool vec, const float2* cs, float (&x)[8]) {
-  const float4 a = load4(p, dtype, head + u.lo, vec), b = load4(p, dtype, head + u.hi, vec);
+  const float4 a = load_row4(p, dtype, head + u.lo, vec), b = load_row4(p, dtype, head + u.hi, vec);
   x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
   if (u.pair < 0 || !cs) return;
 #pragma unroll

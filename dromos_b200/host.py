@@ -278,7 +278,7 @@ class KvBatch:
         if tokens < 0 or max_new < 0:
             raise ValueError("tokens and max_new count from 0")
         self.starts, self.lengths, self.pages, self.tokens, self.max_new = starts, lengths, pages, tokens, max_new
-        self.device = lengths.device
+        self.device, self.sizes = lengths.device, (S, tokens, max_new)
         self.struct = abi.KvBatchStruct(S, tokens, max_new, pages.shape[1], starts.data_ptr(), lengths.data_ptr(), pages.data_ptr())
         self.address = ctypes.addressof(self.struct)
 
@@ -349,9 +349,9 @@ class Attention:
     def __init__(self, cache: KvCache, heads: int, scale: float | None = None, window: int = 0):
         self.cache, self.heads, self.window = cache, heads, window
         self.scale = float(cache.head_dim**-0.5 if scale is None else scale)
-        self._need = {}  # by max_new
-        if cache.lib.lx_b200_attention_workspace_bytes(cache.address, heads, 1) < 0:
-            raise ValueError(f"no attention of {heads} heads over this cache")
+        if heads < 1 or heads % cache.kv_heads:
+            raise ValueError(f"no attention of {heads} heads over a cache of {cache.kv_heads}")
+        self._need = {}  # bytes of workspace, by the sizes they go by
 
     def __call__(self, batch: KvBatch, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """q: f32 or bf16 [tokens, heads * head_dim]; out: bf16, the same shape (rows past the last sequence are left as they are)."""
@@ -365,12 +365,16 @@ class Attention:
         elif out.dtype != torch.bfloat16:
             raise TypeError("out: bfloat16")
         ld_o = _rows(out, T, width, "out", cache.device)
-        need = self._need.get(batch.max_new)
+        need = self._need.get(batch.sizes)
         if need is None:
-            need = self._need[batch.max_new] = cache.lib.lx_b200_attention_workspace_bytes(cache.address, self.heads, batch.max_new)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+            need = cache.lib.lx_b200_attention_workspace_bytes(cache.address, batch.address, self.heads)
+            if need < 0:
+                raise RuntimeError("lx_b200_attention refuses this cache")
+            if len(self._need) < 4096:
+                self._need[batch.sizes] = need
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         st = cache.lib.lx_b200_attention(cache.address, batch.address, q.data_ptr(), dt, ld_q, self.heads, self.scale, self.window, out.data_ptr(), ld_o,
-                                         ws.data_ptr() if need else None, _raw_stream())
+                                         ws.data_ptr(), _raw_stream())
         if st:
             raise RuntimeError(f"lx_b200_attention failed: {st}")
         return out

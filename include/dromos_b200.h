@@ -339,8 +339,9 @@ LX_API int lx_b200_kv_append(const lx_b200_kv_cache* cache, const lx_b200_kv_bat
  * a sequence are cut to even out the work) and are the same every time. */
 LX_API int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q,
                              int q_heads, float scale, int window, void* out, int ld_out, void* workspace, void* stream);
-/* For any batch with this cache's type and head_dim, these q_heads and this max_new; -1 for arguments the call refuses. */
-LX_API int64_t lx_b200_attention_workspace_bytes(const lx_b200_kv_cache* cache, int q_heads, int max_new);
+/* By the cache's head_dim and kv_heads, the batch's sequences, tokens and max_new (its device arrays are not looked at) and the current
+ * device; -1 for arguments the call refuses. */
+LX_API int64_t lx_b200_attention_workspace_bytes(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, int q_heads);
 /* What follows a block and precedes the next, for T rows of C values:
  *   u = y * rsqrt(mean(y^2) + eps) * post        (post null: u = y; y null: u = 0)
  *   h_out = residual_scale * h + block_scale * gate * u      (gate null: 1; gate_sigmoid: 1 / (1 + exp(-gate)))

@@ -86,9 +86,9 @@ def test_appends_that_are_refused(lib):
 def test_attentions_that_are_refused(lib):
     for kw in (dict(q=None), dict(out=None), dict(ld_q=255), dict(ld_out=255), dict(q_dtype=2), dict(q_heads=0), dict(q_heads=5), dict(window=-1), dict(workspace=None), dict(workspace=4104)):
         assert attend(lib, cache(), batch(tokens=4), **kw) == abi.ERR_INVALID, kw
-    assert lib.lx_b200_attention_workspace_bytes(address(cache()), 4, 1) >= 0
-    for args in ((None, 4, 1), (address(cache()), 5, 1), (address(cache()), 0, 1), (address(cache()), 4, -1), (address(cache(head_dim=80)), 4, 1)):
-        assert lib.lx_b200_attention_workspace_bytes(*args) == -1
+    assert lib.lx_b200_attention_workspace_bytes(address(cache()), address(batch()), 4) >= 0
+    for args in ((None, batch(), 4), (cache(), None, 4), (cache(), batch(), 5), (cache(), batch(), 0), (cache(), batch(max_new=-1), 4), (cache(head_dim=80), batch(), 4)):
+        assert lib.lx_b200_attention_workspace_bytes(address(args[0]), address(args[1]), args[2]) == -1
 
 
 def test_norms_that_are_refused(lib):
