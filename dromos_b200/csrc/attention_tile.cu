@@ -38,13 +38,18 @@ struct TileCfg {
   static constexpr int kRowTiles = D == 256 ? 1 : 2;
   static constexpr int kRows = kRowTiles * kRowTile;
   static constexpr int kKeys = D == 256 ? 64 : 128;  // keys of a tile
-  static constexpr int kQBytes = kRowTile * D * 2, kKvBytes = kKeys * D * 2;
-  static constexpr int kRawBytes = kKeys * D;  // a tile's codes
-  static constexpr int kKOff = kRowTiles * kQBytes, kVOff = kKOff + 2 * kKvBytes, kRawOff = kVOff + 2 * kKvBytes, kScaleOff = kRawOff + 2 * kRawBytes;
-  static constexpr int kScaleGroups = kKeys / 16;
-  static constexpr int kBarOff = kScaleOff + 4 * kScaleGroups * 16;
-  static constexpr int kSmem = kBarOff + 256 < 120 * 1024 ? 120 * 1024 : kBarOff + 256;  // one CTA per SM: it takes all of tensor memory
-  static constexpr int kO = 256;  // first column of the accumulators of O; those of S begin at 0
+  static constexpr int kStages = 2, kRawStages = D == 64 ? 2 : 1, kScaleRing = 8;
+  static constexpr int kQBytes = kRowTile * D * 2, kKvBytes = kKeys * D * 2, kRawBytes = kKeys * D;  // a tile: queries, keys or values, their codes
+  static constexpr int kKOff = kRowTiles * kQBytes, kVOff = kKOff + kStages * kKvBytes, kRawOff = kVOff + kStages * kKvBytes;
+  static constexpr int kScaleOff = kRawOff + 2 * kRawStages * kRawBytes, kScaleGroups = kKeys / 16;
+  static constexpr int kBarOff = kScaleOff + kScaleRing * kScaleGroups * 16;
+  static constexpr int kSmem = kBarOff + 512;
+  static constexpr int kO = 256;  // first column of the sums in tensor memory; the scores (and the weights over them) begin at 0
+  static_assert(kRowTiles * kKeys <= kO && kO + kRowTiles * D <= kTmemColumns, "tensor memory");
+  static_assert(kSmem > 116 * 1024 && kSmem <= 226 * 1024, "one CTA per SM: it takes all of tensor memory");
+  // A slot of the scales is written again kScaleRing tiles later: the copies are at most kRawStages + 1 tiles ahead of the widening,
+  // which is at most kStages tiles ahead of the weights that use them.
+  static_assert(kScaleRing >= kStages + kRawStages + 2, "scales");
 };
 
 struct BlockPlan {
@@ -216,47 +221,74 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// A warp's 32 query rows into their core matrices, each times the power of two that brings it into f16's range (and the sign of the
-// softmax's scale); lane r gets the factor of the scores of row r.
+// A thread's query row into its row of the core matrices, times the power of two that brings it into f16's range (and the sign of the
+// softmax's scale); returns the factor of its scores. Read twice: once for its largest magnitude. Rows past the end are zeros.
 template <int D, int DTYPE, bool VEC>
-__device__ __forceinline__ float load_queries(const AttentionArgs& A, const Part& p, int row, uint8_t* to, float sign) {
-  constexpr int V4 = (D + 127) / 128, BATCH = 8 / V4;
-  const int lane = threadIdx.x & 31;
-  float f = 0.0f;
-  int token = row / A.group, head = row % A.group;
-#pragma unroll 1
-  for (int j0 = 0; j0 < 32; j0 += BATCH) {
-    float4 x[BATCH][V4];
+__device__ __forceinline__ float load_query(const AttentionArgs& A, int64_t src, bool there, uint32_t to, float sign) {
+  constexpr int RUN = DTYPE == LX_BF16 && D <= 128 ? D : 32;  // values at once
+  constexpr int PIECES = RUN / 8;
+  float most = 0.0f, up = 1.0f;
+  uint4 raw[PIECES][DTYPE == LX_BF16 ? 1 : 2];
+  auto load = [&](int d0) {
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      // past the last row: its last row's values, so that no load waits for a condition; they are dropped below
-      const int64_t src = (p.q.row0 + min(token, p.q.n - 1)) * A.ld_q + (static_cast<int64_t>(p.head) * A.group + head) * D;
+    for (int i = 0; i < PIECES; ++i) {
+      if constexpr (VEC) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(A.q) + (src + d0 + 8 * i) * (DTYPE == LX_BF16 ? 2 : 4));
+        raw[i][0] = p[0];
+        if constexpr (DTYPE == LX_F32) raw[i][1] = p[1];
+      } else {
+        uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < V4; ++i) x[j][i] = load_row4(A.q, DTYPE < 0 ? A.q_dtype : DTYPE, src + (4 * lane + 128 * i) % D, VEC);
-      if (++head == A.group) head = 0, ++token;
+        for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(load_f32(A.q, A.q_dtype, src + d0 + 8 * i + j));
+        raw[i][0] = make_uint4(w[0], w[1], w[2], w[3]), raw[i][1] = make_uint4(w[4], w[5], w[6], w[7]);
+      }
     }
+  };
+  auto values = [&](int i, float (&v)[8]) {
+    const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
+    if constexpr (DTYPE == LX_BF16) {
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      const bool there = row + j0 + j < p.row_block + p.rows;
-      float most = 0.0f;
+      for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    } else {
+      const uint32_t z[4] = {raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
 #pragma unroll
-      for (int i = 0; i < V4; ++i) {
-        if (!there) x[j][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        most = fmaxf(fmaxf(fmaxf(most, fabsf(x[j][i].x)), fabsf(x[j][i].y)), fmaxf(fabsf(x[j][i].z), fabsf(x[j][i].w)));
-      }
-      const float up = f16_scale(warp_max(most)), by = up * sign;
-      if (lane == j0 + j) f = A.scale_log2 * sign / up;
+      for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(w[j]), v[4 + j] = __uint_as_float(z[j]);
+    }
+  };
+#pragma unroll 1
+  for (int d0 = 0; d0 < D; d0 += RUN) {
+    load(d0);
 #pragma unroll
-      for (int i = 0; i < V4; ++i) {
-        const int d = 4 * lane + 128 * i;
-        const __half2 a = __floats2half2_rn(x[j][i].x * by, x[j][i].y * by), b = __floats2half2_rn(x[j][i].z * by, x[j][i].w * by);
-        if (d < D)
-          *reinterpret_cast<uint2*>(to + d / 8 * (kRowTile * 16) + (j0 + j) * 16 + d % 8 * 2) =
-              make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-      }
+    for (int i = 0; i < PIECES; ++i) {
+      float v[8];
+      values(i, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
     }
   }
-  return f;
+  up = f16_scale(most);
+  const float by = there ? up * sign : 0.0f;
+#pragma unroll 1
+  for (int d0 = 0; d0 < D; d0 += RUN) {
+    if constexpr (RUN < D) load(d0);
+#pragma unroll
+    for (int h = 0; h < RUN / 32; ++h) {
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v[8];
+        values(4 * h + i, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __half2 x = __floats2half2_rn(there ? v[2 * j] * by : 0.0f, there ? v[2 * j + 1] * by : 0.0f);
+          w[4 * i + j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sts128(to + (d0 / 8 + 4 * h + i) * (kRowTile * 16), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+  }
+  return A.scale_log2 * sign / up;
 }
 
 // Eight results; whole: they lie on 16 bytes.
@@ -370,20 +402,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   const AttentionArgs& A = T.a;
   const KvView& V = A.kv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int NS = C::kStages, RS = C::kRawStages;
   const uint32_t q_base = smem_u32(smem), k_base = q_base + C::kKOff, v_base = q_base + C::kVOff, raw_base = q_base + C::kRawOff, bars = q_base + C::kBarOff;
-  float4* const scales = reinterpret_cast<float4*>(smem + C::kScaleOff);  // [4][kScaleGroups]: kscale, log2 vscale, 2^-shift / vscale
-  const uint32_t q_full = bars, s_full = bars + 16, p_full = bars + 32, k_full = bars + 48, k_empty = bars + 64, v_full = bars + 80, v_empty = bars + 96,
-                 raw_full = bars + 112, raw_empty = bars + 128;  // raw: keys', values'
+  float4* const scales = reinterpret_cast<float4*>(smem + C::kScaleOff);  // [ring][group of 16 slots]: kscale, log2 vscale, 2^-shift / vscale, 1 with codes
+  // per row tile: queries in, scores done, weights in, sums done; per stage: keys and values in and read; codes in and read (keys' two
+  // stages, values' two)
+  const uint32_t q_full = bars, s_full = bars + 16, p_full = bars + 32, o_full = bars + 48, raw_full = bars + 64, raw_empty = bars + 96, k_full = bars + 128,
+                 k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + 8 * i, kRowTile);
       mbar_init(s_full + 8 * i, 1);
       mbar_init(p_full + 8 * i, kRowTile);
+      mbar_init(o_full + 8 * i, 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(raw_full + 8 * i, 32);
+      mbar_init(raw_empty + 8 * i, 32 * kWidenWarps);
+    }
+    for (int i = 0; i < NS; ++i) {
       mbar_init(k_full + 8 * i, 32 * kWidenWarps);
       mbar_init(k_empty + 8 * i, 1);
       mbar_init(v_full + 8 * i, 32 * kWidenWarps);
-      mbar_init(raw_full + 8 * i, 32);
-      mbar_init(raw_empty + 8 * i, 32 * kWidenWarps);
       mbar_init(v_empty + 8 * i, 1);
     }
     mbar_init_fence();
@@ -417,48 +457,49 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       // 128 bytes between groups of 8 rows above
       const uint32_t desc_hi = (128u >> 4) | (1u << 14);
       uint32_t kn = 0, vn = 0, qn[2] = {0, 0}, pn[2] = {0, 0};
-      bool ok = true;
       auto scores = [&](int rt) {
-        const uint32_t qa = (q_base + rt * C::kQBytes) >> 4 | kRowTile << 16, kb = (k_base + (kn & 1) * C::kKvBytes) >> 4 | KT << 16;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-          umma_ss_halves<kActF16>(tmem + rt * KT, qa + i * 2 * kRowTile, desc_hi, kb + i * 2 * KT, desc_hi, idesc_s, i > 0);
+        uint32_t qa = (q_base + rt * C::kQBytes) >> 4 | kRowTile << 16, kb = (k_base + kn % NS * C::kKvBytes) >> 4 | KT << 16;
+        // rolled: these few instructions come from the instruction cache while the softmax's thousands go through it (unrolled, an
+        // instruction took 150 cycles to issue)
+#pragma unroll 1
+        for (int i = 0; i < D / 16; ++i, qa += 2 * kRowTile, kb += 2 * KT) umma_ss_halves<kActF16>(tmem + rt * KT, qa, desc_hi, kb, desc_hi, idesc_s, i > 0);
+        umma_commit(s_full + 8 * rt);
       };
-      while (ok && next_part<C::kRows>(T, share, p)) {
-        const int tiles_of_rows = p.rows > kRowTile ? 2 : 1;
-        if (!tc_wait(k_full + 8 * (kn & 1), kn >> 1 & 1, V.status)) break;
+      bool more_parts = next_part<C::kRows>(T, share, p), ok = true;
+      while (ok && more_parts) {
+        const int tiles_of_rows = p.rows > kRowTile ? 2 : 1, tiles = p.tiles;
+        if (!tc_wait(k_full + 8 * (kn % NS), kn / NS & 1, V.status)) break;
         for (int rt = 0; rt < tiles_of_rows && ok; ++rt) {
           ok = tc_wait(q_full + 8 * rt, qn[rt]++ & 1, V.status);
           if (!ok) break;
           tc_fence_after();
           scores(rt);
-          umma_commit(s_full + 8 * rt);
         }
         if (!ok) break;
-        umma_commit(k_empty + 8 * (kn & 1));
+        umma_commit(k_empty + 8 * (kn % NS));
         ++kn;
-        for (int i = 0; i < p.tiles && ok; ++i) {
-          const bool more = i + 1 < p.tiles;
+        more_parts = next_part<C::kRows>(T, share, p);
+        for (int i = 0; i < tiles && ok; ++i) {
+          const bool more = i + 1 < tiles;
           for (int rt = 0; rt < tiles_of_rows; ++rt) {
-            if ((rt == 0 && !tc_wait(v_full + 8 * (vn & 1), vn >> 1 & 1, V.status)) || !tc_wait(p_full + 8 * rt, pn[rt] & 1, V.status) ||
-                (rt == 0 && more && !tc_wait(k_full + 8 * (kn & 1), kn >> 1 & 1, V.status))) {
+            if ((rt == 0 && !tc_wait(v_full + 8 * (vn % NS), vn / NS & 1, V.status)) || !tc_wait(p_full + 8 * rt, pn[rt] & 1, V.status) ||
+                (rt == 0 && more && !tc_wait(k_full + 8 * (kn % NS), kn / NS & 1, V.status))) {
               ok = false;
               break;
             }
             ++pn[rt];
             tc_fence_after();
-            const uint32_t vb = (v_base + (vn & 1) * C::kKvBytes) >> 4 | D << 16;
-#pragma unroll
-            for (int j = 0; j < KT / 16; ++j)
-              umma_ts(tmem + C::kO + rt * D, tmem + rt * KT + 8 * j, vb + j * 2 * D, desc_hi, idesc_o, i > 0 || j > 0);
+            uint32_t vb = (v_base + vn % NS * C::kKvBytes) >> 4 | D << 16;
+#pragma unroll 1
+            for (int j = 0; j < KT / 16; ++j, vb += 2 * D) umma_ts(tmem + C::kO + rt * D, tmem + rt * KT + 8 * j, vb, desc_hi, idesc_o, i > 0 || j > 0);
             if (more) scores(rt);
-            umma_commit(s_full + 8 * rt);  // the next scores, or, after the last tile, the sums
+            else umma_commit(o_full + 8 * rt);
           }
           if (!ok) break;
-          umma_commit(v_empty + 8 * (vn & 1));
+          umma_commit(v_empty + 8 * (vn % NS));
           ++vn;
           if (more) {
-            umma_commit(k_empty + 8 * (kn & 1));
+            umma_commit(k_empty + 8 * (kn % NS));
             ++kn;
           }
         }
@@ -487,25 +528,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
               const float v = V.v_scale[at], vs = v < 0x1p-100f ? 0x1p-100f : v;
               s = make_float4(V.k_scale[at], __log2f(vs), kUnshift / vs, 1.0f);
             }
-            scales[(n & 3) * C::kScaleGroups + lane] = s;
+            scales[n % C::kScaleRing * C::kScaleGroups + lane] = s;
           }
           for (int kv = 0; kv < 2 && ok; ++kv) {
-            ok = tc_wait(raw_empty + 8 * kv, (n & 1) ^ 1, V.status);
+            const uint32_t at = RS * kv + n % RS;
+            ok = tc_wait(raw_empty + 8 * at, (n / RS & 1) ^ 1, V.status);
             if (!ok) break;
-            const uint32_t bar = raw_full + 8 * kv;
             if (page >= 0) {
-              mbar_arrive_expect_tx(bar, 16 * D);
-              bulk_g2s(raw_base + kv * C::kRawBytes + 16 * lane * D, (kv ? V.v : V.k) + src, 16 * D, bar);
+              mbar_arrive_expect_tx(raw_full + 8 * at, 16 * D);
+              bulk_g2s(raw_base + at * C::kRawBytes + 16 * lane * D, (kv ? V.v : V.k) + src, 16 * D, raw_full + 8 * at);
             } else {
-              mbar_arrive(bar);
+              mbar_arrive(raw_full + 8 * at);
             }
             ++sent[kv];
           }
         }
       }
-      // copies in flight end before the CTA does
+      // copies in flight end before the CTA does: the last ones of each kind
       for (int kv = 0; kv < 2; ++kv)
-        if (sent[kv] > 0) tc_wait(raw_full + 8 * kv, (sent[kv] - 1) & 1, V.status);
+        for (uint32_t i = sent[kv] > RS ? sent[kv] - RS : 0; i < sent[kv]; ++i) tc_wait(raw_full + 8 * (RS * kv + i % RS), i / RS & 1, V.status);
     }
   } else if (warp < kSoftmaxWarps) {
     // ================================ softmax: a row per thread ================================
@@ -513,26 +554,37 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     const int rt = warp >> 2, row = tid & (kRowTile - 1);
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_tmem = tmem + lanes + rt * KT, o_tmem = tmem + lanes + C::kO + rt * D;
-    uint32_t sn = 0, tiles_done = 0;
+    uint32_t sn = 0, on = 0, tiles_done = 0;
     bool ok = true;
     const float sign = A.scale_log2 < 0.0f ? -1.0f : 1.0f;
-    while (ok && next_part<C::kRows>(T, share, p)) {
+    Part next;
+    bool more_parts = next_part<C::kRows>(T, share, next);
+    float f = 0.0f;
+    // the queries of a part, as soon as the scores of the part before are done
+    auto queries = [&]() {
+      const int r = next.row_block + rt * kRowTile + row;
+      const bool there = r < next.row_block + next.rows;
+      const int q = there ? r : next.row_block + next.rows - 1;  // a row that is there, for the loads
+      const int64_t src = (next.q.row0 + q / A.group) * A.ld_q + (static_cast<int64_t>(next.head) * A.group + q % A.group) * D;
+      const uint32_t to = q_base + rt * C::kQBytes + row * 16;
+      if (T.q_vec && A.q_dtype == LX_BF16) f = load_query<D, LX_BF16, true>(A, src, there, to, sign);
+      else if (T.q_vec) f = load_query<D, LX_F32, true>(A, src, there, to, sign);
+      else f = load_query<D, -1, false>(A, src, there, to, sign);
+      proxy_fence();
+      mbar_arrive(q_full + 8 * rt);
+    };
+    auto takes = [&](const Part& x) { return rt < RT && (rt == 0 || x.rows > kRowTile); };
+    if (more_parts && takes(next)) queries();
+    while (ok && more_parts) {
+      p = next;
       const int first = p.q.length - p.q.n, row0 = p.row_block + rt * kRowTile;
-      const bool mine = rt < RT && (rt == 0 || p.rows > kRowTile);
-      float f = 0.0f;
-      if (mine) {
-        // the rows of this warp's lanes, each times the power of two that brings it into f16's range
-        const int w_row = 32 * (warp & 3);
-        if (T.q_vec && A.q_dtype == LX_BF16) f = load_queries<D, LX_BF16, true>(A, p, row0 + w_row, smem + rt * C::kQBytes + w_row * 16, sign);
-        else if (T.q_vec) f = load_queries<D, LX_F32, true>(A, p, row0 + w_row, smem + rt * C::kQBytes + w_row * 16, sign);
-        else f = load_queries<D, -1, false>(A, p, row0 + w_row, smem + rt * C::kQBytes + w_row * 16, sign);
-        proxy_fence();
-        mbar_arrive(q_full + 8 * rt);
-      }
-      if (!mine) {
+      if (!takes(p)) {
         tiles_done += p.tiles;
+        more_parts = next_part<C::kRows>(T, share, next);
+        if (more_parts && takes(next)) queries();
         continue;
       }
+      const float f_now = f;
       const int r = row0 + row;
       const bool valid = r < p.row_block + p.rows;
       const int past = valid ? first + r / A.group + 1 : 0;
@@ -541,7 +593,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       float m = -INFINITY, l = 0.0f;
       for (int i = 0; i < p.tiles; ++i) {
         const int key0 = (p.tile + i) * KT;
-        const float4* sc = scales + ((tiles_done + i) & 3) * C::kScaleGroups;
+        const float4* sc = scales + (tiles_done + i) % C::kScaleRing * C::kScaleGroups;
         if (!tc_wait(s_full + 8 * rt, sn & 1, V.status)) {
           ok = false;
           break;
@@ -558,9 +610,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         float top;
         if (edge) {
           mask_scores<true, KT>(u, lo, hi);
-          top = tile_top<true, KT>(u, sc, f);
+          top = tile_top<true, KT>(u, sc, f_now);
         } else {
-          top = tile_top<false, KT>(u, sc, f);
+          top = tile_top<false, KT>(u, sc, f_now);
         }
         const bool higher = top > m + kSlack;  // at first m is -inf
         if (__any_sync(0xffffffffu, higher)) {
@@ -581,17 +633,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           }
         }
         const float from = (m == -INFINITY ? 0.0f : m) - kShift;
-        l += edge ? tile_weights<true, KT>(u, s_tmem, sc, f, from) : tile_weights<false, KT>(u, s_tmem, sc, f, from);
+        l += edge ? tile_weights<true, KT>(u, s_tmem, sc, f_now, from) : tile_weights<false, KT>(u, s_tmem, sc, f_now, from);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_full + 8 * rt);
+        if (i == 0) more_parts = next_part<C::kRows>(T, share, next);
       }
       tiles_done += p.tiles;
-      if (!ok || !tc_wait(s_full + 8 * rt, sn & 1, V.status)) {
+      if (!ok) break;
+      if (more_parts && takes(next)) queries();
+      if (!tc_wait(o_full + 8 * rt, on & 1, V.status)) {
         ok = false;
         break;
       }
-      ++sn;
+      ++on;
       __syncwarp();
       tc_fence_after();
       float* const part = T.partial + (2 * static_cast<int64_t>(blockIdx.x) + p.starts) * (C::kRows * (D + 2));
@@ -631,29 +686,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs));
     const int w4 = warp & 3;
     constexpr int WK = KT / 4;  // slots of a tile that one warp has
-    const uint8_t* const raw_k = smem + C::kRawOff;
-    const uint8_t* const raw_v = raw_k + C::kRawBytes;
     uint32_t n = 0;
     bool ok = true;
     while (ok && next_part<C::kRows>(T, share, p)) {
       for (int i = 0; i < p.tiles && ok; ++i, ++n) {
         const int slot0 = (p.tile + i) * KT;
         const bool all = slot0 >= p.see_low && slot0 + KT <= p.past_high;  // else what no row sees, which was not copied, reads as 0
+        const uint8_t* const raw_k = smem + C::kRawOff + n % RS * C::kRawBytes;
+        const uint8_t* const raw_v = raw_k + RS * C::kRawBytes;
         auto seen = [&](int j) { return all || (slot0 + j < p.past_high && slot0 + j >= p.see_low); };
         // keys. Lane i of eight takes key i of a run, and of its pieces of 16 bytes another one than its neighbours: neither the reads of
         // rows nor the writes of core matrices meet in a bank
-        if (!tc_wait(raw_full, n & 1, V.status) || !tc_wait(k_empty + 8 * (n & 1), (n >> 1 & 1) ^ 1, V.status)) {
+        if (!tc_wait(raw_full + 8 * (n % RS), n / RS & 1, V.status) || !tc_wait(k_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
           ok = false;
           break;
         }
         {
           constexpr int PIECES = D / 16;
-          const uint32_t dst = k_base + (n & 1) * C::kKvBytes;
+          const uint32_t dst = k_base + n % NS * C::kKvBytes;
           const int key8 = lane & 7;
-#pragma unroll
+#pragma unroll 1
           for (int a = 0; a < WK / 8; ++a) {
             const int key = w4 * WK + 8 * a + key8;
-            const bool use = seen(key) && scales[(n & 3) * C::kScaleGroups + key / 16].w != 0.0f;
+            const bool use = seen(key) && scales[n % C::kScaleRing * C::kScaleGroups + key / 16].w != 0.0f;
 #pragma unroll
             for (int b = 0; b < PIECES / 4; ++b) {
               const int piece = ((D == 64 ? key8 >> 1 : key8) + 4 * b + (lane >> 3)) & (PIECES - 1);
@@ -669,22 +724,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             }
           }
         }
-        mbar_arrive(raw_empty);
+        mbar_arrive(raw_empty + 8 * (n % RS));
         proxy_fence();
-        mbar_arrive(k_full + 8 * (n & 1));
+        mbar_arrive(k_full + 8 * (n % NS));
         // values: lane: four dims of eight keys; with 64 values per head the half warps have a run of eight keys each
-        if (!tc_wait(raw_full + 8, n & 1, V.status) || !tc_wait(v_empty + 8 * (n & 1), (n >> 1 & 1) ^ 1, V.status)) {
+        if (!tc_wait(raw_full + 8 * (RS + n % RS), n / RS & 1, V.status) || !tc_wait(v_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
           ok = false;
           break;
         }
         {
           constexpr int LANES = D < 128 ? D / 4 : 32, AT_ONCE = 32 / LANES, RUNS = WK / (8 * AT_ONCE), HALVES = D > 128 ? 2 : 1;
           const int l = lane % LANES, sub = lane / LANES;
-          const uint32_t dst = v_base + (n & 1) * C::kKvBytes;
-#pragma unroll
+          const uint32_t dst = v_base + n % NS * C::kKvBytes;
+#pragma unroll 1
           for (int a = 0; a < RUNS; ++a) {
             const int run = w4 * (WK / 8) + a * AT_ONCE + sub;
-            const bool use = scales[(n & 3) * C::kScaleGroups + run / 2].w != 0.0f;
+            const bool use = scales[n % C::kScaleRing * C::kScaleGroups + run / 2].w != 0.0f;
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) {
               uint32_t x[8], o[4][4];  // o: dim, pair of keys
@@ -704,9 +759,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             }
           }
         }
-        mbar_arrive(raw_empty + 8);
+        mbar_arrive(raw_empty + 8 * (RS + n % RS));
         proxy_fence();
-        mbar_arrive(v_full + 8 * (n & 1));
+        mbar_arrive(v_full + 8 * (n % NS));
       }
     }
   }
@@ -794,7 +849,7 @@ int tile_attention(AttentionArgs A, int head_dim, bool int8, int limit, void* wo
   T.header = reinterpret_cast<PlanHeader*>(ws), T.plan = reinterpret_cast<BlockPlan*>(ws + L.plan), T.partial = reinterpret_cast<float*>(ws + L.partial);
   T.capacity = L.capacity;
   T.out_vec8 = aligned(A.out, 16) && A.ld_out % 8 == 0;
-  T.q_vec = aligned(A.q, A.q_dtype == LX_BF16 ? 8 : 16) && A.ld_q % 4 == 0;
+  T.q_vec = aligned(A.q, 16) && A.ld_q % (A.q_dtype == LX_BF16 ? 8 : 4) == 0;
   switch (head_dim) {
     case 64: return int8 ? launch_tile<true, 64>(T, stream) : launch_tile<false, 64>(T, stream);
     case 128: return int8 ? launch_tile<true, 128>(T, stream) : launch_tile<false, 128>(T, stream);
