@@ -216,6 +216,20 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32
       "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// One arrival for a warp, after all of its lanes: 128 arrivals of a role's threads take their turns at the barrier for as long as a
+// tile's products take.
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+  return one != 0;
+}
+// A wait of a whole warp: where one lane gives up all of them do.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* status) { return __all_sync(0xffffffffu, tc_wait(bar, parity, status)); }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -411,19 +425,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                  k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full + 8 * i, kRowTile);
+      mbar_init(q_full + 8 * i, 4);
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_full + 8 * i, kRowTile);
+      mbar_init(p_full + 8 * i, 4);
       mbar_init(o_full + 8 * i, 1);
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(raw_full + 8 * i, 32);
-      mbar_init(raw_empty + 8 * i, 32 * kWidenWarps);
+      mbar_init(raw_full + 8 * i, 1);
+      mbar_init(raw_empty + 8 * i, kWidenWarps);
     }
     for (int i = 0; i < NS; ++i) {
-      mbar_init(k_full + 8 * i, 32 * kWidenWarps);
+      mbar_init(k_full + 8 * i, kWidenWarps);
       mbar_init(k_empty + 8 * i, 1);
-      mbar_init(v_full + 8 * i, 32 * kWidenWarps);
+      mbar_init(v_full + 8 * i, kWidenWarps);
       mbar_init(v_empty + 8 * i, 1);
     }
     mbar_init_fence();
@@ -450,7 +464,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   if (warp >= kMmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
     // ================================ the products ================================
-    if (warp == kMmaWarp && lane == 0) {
+    if (warp == kMmaWarp) {
+      // The whole warp goes through the loops, one lane issues: what the instructions take is then the same in all lanes and stays in
+      // uniform registers. (One lane alone in the loops took 115 cycles for each product, whose own time is 66.)
       const uint32_t idesc_s = (1u << 4) | (static_cast<uint32_t>(KT >> 3) << 17) | (static_cast<uint32_t>(kRowTile >> 4) << 24);
       const uint32_t idesc_o = (1u << 4) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kRowTile >> 4) << 24);
       // descriptors of core matrices (smem_desc): address and the step along the summed dimension, both in 16 bytes, below; the step of
@@ -458,50 +474,58 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       const uint32_t desc_hi = (128u >> 4) | (1u << 14);
       uint32_t kn = 0, vn = 0, qn[2] = {0, 0}, pn[2] = {0, 0};
       auto scores = [&](int rt) {
-        uint32_t qa = (q_base + rt * C::kQBytes) >> 4 | kRowTile << 16, kb = (k_base + kn % NS * C::kKvBytes) >> 4 | KT << 16;
-        // rolled: these few instructions come from the instruction cache while the softmax's thousands go through it (unrolled, an
-        // instruction took 150 cycles to issue)
-#pragma unroll 1
-        for (int i = 0; i < D / 16; ++i, qa += 2 * kRowTile, kb += 2 * KT) umma_ss_halves<kActF16>(tmem + rt * KT, qa, desc_hi, kb, desc_hi, idesc_s, i > 0);
-        umma_commit(s_full + 8 * rt);
+        const uint32_t qa = (q_base + rt * C::kQBytes) >> 4 | kRowTile << 16, kb = (k_base + kn % NS * C::kKvBytes) >> 4 | KT << 16;
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            umma_ss_halves<kActF16>(tmem + rt * KT, qa + i * 2 * kRowTile, desc_hi, kb + i * 2 * KT, desc_hi, idesc_s, i > 0);
+          umma_commit(s_full + 8 * rt);
+        }
+        __syncwarp();
       };
       bool more_parts = next_part<C::kRows>(T, share, p), ok = true;
       while (ok && more_parts) {
         const int tiles_of_rows = p.rows > kRowTile ? 2 : 1, tiles = p.tiles;
-        if (!tc_wait(k_full + 8 * (kn % NS), kn / NS & 1, V.status)) break;
+        if (!warp_wait(k_full + 8 * (kn % NS), kn / NS & 1, V.status)) break;
         for (int rt = 0; rt < tiles_of_rows && ok; ++rt) {
-          ok = tc_wait(q_full + 8 * rt, qn[rt]++ & 1, V.status);
+          ok = warp_wait(q_full + 8 * rt, qn[rt]++ & 1, V.status);
           if (!ok) break;
           tc_fence_after();
           scores(rt);
         }
         if (!ok) break;
-        umma_commit(k_empty + 8 * (kn % NS));
+        if (elect_one()) umma_commit(k_empty + 8 * (kn % NS));
+        __syncwarp();
         ++kn;
         more_parts = next_part<C::kRows>(T, share, p);
         for (int i = 0; i < tiles && ok; ++i) {
           const bool more = i + 1 < tiles;
           for (int rt = 0; rt < tiles_of_rows; ++rt) {
-            if ((rt == 0 && !tc_wait(v_full + 8 * (vn % NS), vn / NS & 1, V.status)) || !tc_wait(p_full + 8 * rt, pn[rt] & 1, V.status) ||
-                (rt == 0 && more && !tc_wait(k_full + 8 * (kn % NS), kn / NS & 1, V.status))) {
+            if ((rt == 0 && !warp_wait(v_full + 8 * (vn % NS), vn / NS & 1, V.status)) || !warp_wait(p_full + 8 * rt, pn[rt] & 1, V.status) ||
+                (rt == 0 && more && !warp_wait(k_full + 8 * (kn % NS), kn / NS & 1, V.status))) {
               ok = false;
               break;
             }
             ++pn[rt];
             tc_fence_after();
-            uint32_t vb = (v_base + vn % NS * C::kKvBytes) >> 4 | D << 16;
-#pragma unroll 1
-            for (int j = 0; j < KT / 16; ++j, vb += 2 * D) umma_ts(tmem + C::kO + rt * D, tmem + rt * KT + 8 * j, vb, desc_hi, idesc_o, i > 0 || j > 0);
+            const uint32_t vb = (v_base + vn % NS * C::kKvBytes) >> 4 | D << 16;
+            if (elect_one()) {
+#pragma unroll
+              for (int j = 0; j < KT / 16; ++j)
+                umma_ts(tmem + C::kO + rt * D, tmem + rt * KT + 8 * j, vb + j * 2 * D, desc_hi, idesc_o, i > 0 || j > 0);
+              if (!more) umma_commit(o_full + 8 * rt);
+            }
+            __syncwarp();
             if (more) scores(rt);
-            else umma_commit(o_full + 8 * rt);
           }
           if (!ok) break;
-          umma_commit(v_empty + 8 * (vn % NS));
-          ++vn;
-          if (more) {
-            umma_commit(k_empty + 8 * (kn % NS));
-            ++kn;
+          if (elect_one()) {
+            umma_commit(v_empty + 8 * (vn % NS));
+            if (more) umma_commit(k_empty + 8 * (kn % NS));
           }
+          __syncwarp();
+          ++vn;
+          kn += more;
         }
       }
     }
@@ -532,14 +556,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           }
           for (int kv = 0; kv < 2 && ok; ++kv) {
             const uint32_t at = RS * kv + n % RS;
-            ok = tc_wait(raw_empty + 8 * at, (n / RS & 1) ^ 1, V.status);
+            ok = warp_wait(raw_empty + 8 * at, (n / RS & 1) ^ 1, V.status);
             if (!ok) break;
-            if (page >= 0) {
-              mbar_arrive_expect_tx(raw_full + 8 * at, 16 * D);
-              bulk_g2s(raw_base + at * C::kRawBytes + 16 * lane * D, (kv ? V.v : V.k) + src, 16 * D, raw_full + 8 * at);
-            } else {
-              mbar_arrive(raw_full + 8 * at);
-            }
+            __syncwarp();
+            const uint32_t copies = __ballot_sync(0xffffffffu, page >= 0);
+            if (lane == 0) mbar_arrive_expect_tx(raw_full + 8 * at, __popc(copies) * 16 * D);
+            __syncwarp();
+            if (page >= 0) bulk_g2s(raw_base + at * C::kRawBytes + 16 * lane * D, (kv ? V.v : V.k) + src, 16 * D, raw_full + 8 * at);
             ++sent[kv];
           }
         }
@@ -571,7 +594,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       else if (T.q_vec) f = load_query<D, LX_F32, true>(A, src, there, to, sign);
       else f = load_query<D, -1, false>(A, src, there, to, sign);
       proxy_fence();
-      mbar_arrive(q_full + 8 * rt);
+      warp_arrive(q_full + 8 * rt);
     };
     auto takes = [&](const Part& x) { return rt < RT && (rt == 0 || x.rows > kRowTile); };
     if (more_parts && takes(next)) queries();
@@ -594,12 +617,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       for (int i = 0; i < p.tiles; ++i) {
         const int key0 = (p.tile + i) * KT;
         const float4* sc = scales + (tiles_done + i) % C::kScaleRing * C::kScaleGroups;
-        if (!tc_wait(s_full + 8 * rt, sn & 1, V.status)) {
+        if (!warp_wait(s_full + 8 * rt, sn & 1, V.status)) {
           ok = false;
           break;
         }
         ++sn;
-        __syncwarp();
         tc_fence_after();
         const bool edge = key0 + KT > past_low || key0 < see_all;
         const int lo = low - key0, hi = past - key0;
@@ -636,18 +658,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         l += edge ? tile_weights<true, KT>(u, s_tmem, sc, f_now, from) : tile_weights<false, KT>(u, s_tmem, sc, f_now, from);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(p_full + 8 * rt);
+        warp_arrive(p_full + 8 * rt);
         if (i == 0) more_parts = next_part<C::kRows>(T, share, next);
       }
       tiles_done += p.tiles;
       if (!ok) break;
       if (more_parts && takes(next)) queries();
-      if (!tc_wait(o_full + 8 * rt, on & 1, V.status)) {
+      if (!warp_wait(o_full + 8 * rt, on & 1, V.status)) {
         ok = false;
         break;
       }
       ++on;
-      __syncwarp();
       tc_fence_after();
       float* const part = T.partial + (2 * static_cast<int64_t>(blockIdx.x) + p.starts) * (C::kRows * (D + 2));
       const int pr = rt * kRowTile + row;
@@ -697,7 +718,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         auto seen = [&](int j) { return all || (slot0 + j < p.past_high && slot0 + j >= p.see_low); };
         // keys. Lane i of eight takes key i of a run, and of its pieces of 16 bytes another one than its neighbours: neither the reads of
         // rows nor the writes of core matrices meet in a bank
-        if (!tc_wait(raw_full + 8 * (n % RS), n / RS & 1, V.status) || !tc_wait(k_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
+        if (!warp_wait(raw_full + 8 * (n % RS), n / RS & 1, V.status) || !warp_wait(k_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
           ok = false;
           break;
         }
@@ -724,11 +745,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             }
           }
         }
-        mbar_arrive(raw_empty + 8 * (n % RS));
+        warp_arrive(raw_empty + 8 * (n % RS));
         proxy_fence();
-        mbar_arrive(k_full + 8 * (n % NS));
+        warp_arrive(k_full + 8 * (n % NS));
         // values: lane: four dims of eight keys; with 64 values per head the half warps have a run of eight keys each
-        if (!tc_wait(raw_full + 8 * (RS + n % RS), n / RS & 1, V.status) || !tc_wait(v_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
+        if (!warp_wait(raw_full + 8 * (RS + n % RS), n / RS & 1, V.status) || !warp_wait(v_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
           ok = false;
           break;
         }
@@ -759,9 +780,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             }
           }
         }
-        mbar_arrive(raw_empty + 8 * (RS + n % RS));
+        warp_arrive(raw_empty + 8 * (RS + n % RS));
         proxy_fence();
-        mbar_arrive(v_full + 8 * (n % NS));
+        warp_arrive(v_full + 8 * (n % NS));
       }
     }
   }
