@@ -511,7 +511,7 @@ extern "C" int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv
   if (!valid_dtype(q_dtype) || q_heads < 1 || q_heads % cache->kv_heads || window < 0 || width > INT_MAX) return kInvalid;
   if (batch->sequences == 0 || batch->tokens == 0) return kOk;
   if (static_cast<int64_t>(batch->tokens) * (q_heads / cache->kv_heads) > INT_MAX / 2) return kNotSupported;
-  if (!q || !out || ld_q < width || ld_out < width || !workspace || !aligned(workspace, 16)) return kInvalid;
+  if (!q || !out || ld_q < width || ld_out < width || !workspace || !aligned(workspace, 256)) return kInvalid;
   AttentionArgs A;
   A.kv = view_of(*cache, *batch);
   A.q = q, A.out = static_cast<uint16_t*>(out), A.ld_q = ld_q, A.ld_out = ld_out, A.partial = static_cast<float*>(workspace);

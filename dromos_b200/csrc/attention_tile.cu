@@ -6,8 +6,7 @@
 //
 // A CTA takes 256 rows (128 where a head has 256 values) of one sequence and key head, a row being a new token and one of the heads that
 // share the keys, in two tiles of 128: S = Q K^T of one tile runs while the other's softmax does. Roles: two groups of four warps each
-// have a row per thread, hold its 128 scores in registers and write the weights back over them in tensor memory, as the first
-// operand of O += P V; one warp brings codes and scales in (bulk copies of 16 slots, so pages of any size); four warps widen keys and
+// have a row per thread, read its scores from tensor memory and write the weights back over them, as the first operand of O += P V; one warp brings codes and scales in (bulk copies of 16 slots, so pages of any size); four warps widen keys and
 // values (values transposed: both operands of both products lie along the summed dimension, in core matrices of 8 x 16 bytes); one
 // thread issues the products. Values are stored with dim 4 l + j at n = 32 j + l, so that the four dims of a loaded word go to four
 // conflict-free stores; results are put back in order as they are read.
@@ -27,9 +26,9 @@ constexpr int kSoftmaxWarps = 8, kWidenWarps = 4;
 constexpr int kMmaWarp = kSoftmaxWarps + kWidenWarps, kLoadWarp = kMmaWarp + 1;
 constexpr int kTileThreads = 32 * (kMmaWarp + 4);  // whole groups of four warps, each with its own share of the registers
 // Registers a thread: 128 at launch (512 threads), 65,536 in all; 256 x kSoftmaxRegs + 128 x kWidenRegs + 128 x kMmaRegs are as many.
-constexpr int kSoftmaxRegs = 192, kWidenRegs = 80, kMmaRegs = 48;
+constexpr int kSoftmaxRegs = 160, kWidenRegs = 96, kMmaRegs = 96;
 static_assert(256 * kSoftmaxRegs + 128 * kWidenRegs + 128 * kMmaRegs <= 512 * 128, "more registers than the launch has");
-constexpr int kBlockCost = 3;
+constexpr int kBlockCost = 4;
 constexpr int kShift = 12;  // the largest weights are 2^12 .. 2^15
 constexpr float kSlack = 3.0f, kUnshift = 0x1p-12f;
 
@@ -68,7 +67,7 @@ struct TileArgs {
   BlockPlan* plan;
   float* partial;
   int capacity;  // blocks that `plan` has room for
-  bool q_vec, out_vec8;
+  bool q_vec, out_whole;
 };
 
 // ---- the order of work -----------------------------------------------------------------------------------------------------
@@ -305,15 +304,22 @@ __device__ __forceinline__ float load_query(const AttentionArgs& A, int64_t src,
   return A.scale_log2 * sign / up;
 }
 
-// Eight results; whole: they lie on 16 bytes.
-__device__ __forceinline__ void store_out8(const AttentionArgs& A, int64_t at, const float4& a, const float4& b, float factor, bool whole) {
-  if (!whole) {
-    store_out(A, at, a, factor);
-    store_out(A, at + 4, b, factor);
-    return;
+// Sixteen results, or sums, of a row; whole: they lie on 32 bytes.
+__device__ __forceinline__ void store8(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
+               "r"(w[7])
+               : "memory");
+}
+__device__ __forceinline__ void store_out16(const AttentionArgs& A, int64_t at, const float (&v)[16], float factor, bool whole) {
+  if (whole) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = f32_to_bf16_bits(v[2 * i] * factor) | f32_to_bf16_bits(v[2 * i + 1] * factor) << 16;
+    store8(A.out + at, w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) store_out(A, at + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]), factor);
   }
-  auto two = [&](float x, float y) { return f32_to_bf16_bits(x * factor) | f32_to_bf16_bits(y * factor) << 16; };
-  *reinterpret_cast<uint4*>(A.out + at) = make_uint4(two(a.x, a.y), two(a.z, a.w), two(b.x, b.y), two(b.z, b.w));
 }
 
 // ---- one row's softmax over a tile of scores -------------------------------------------------------------------------------------
@@ -336,72 +342,90 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// A row's scores of a tile, from tensor memory. EDGE: some row of the warps does not see all of it; this one sees the slots
-// lo <= j < hi of the tile.
-template <bool EDGE, int KT>
-__device__ __forceinline__ void mask_scores(uint32_t (&u)[KT / 32][32], int lo, int hi) {
+// EDGE: some row of the warps does not see all of a tile; this one sees its slots lo <= j < hi. The loops stay rolled and read the
+// scores from tensor memory 32 at a time, the next ones while these are worked on: 128 scores in registers and straight code for
+// them ran at the rate of the instruction cache (a tile's weights 2100 cycles).
+template <bool EDGE>
+__device__ __forceinline__ void mask_scores(uint32_t (&u)[32], int at, int lo, int hi) {
   if constexpr (EDGE) {
 #pragma unroll
-    for (int c = 0; c < KT / 32; ++c)
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (32 * c + j >= hi || 32 * c + j < lo) u[c][j] = 0xff800000u;
+    for (int j = 0; j < 32; ++j)
+      if (at + j >= hi || at + j < lo) u[j] = 0xff800000u;
   }
 }
 // The largest t of a tile.
 template <bool EDGE, int KT>
-__device__ __forceinline__ float tile_top(const uint32_t (&u)[KT / 32][32], const float4* sc, float f) {
+__device__ __forceinline__ float tile_top(uint32_t s_tmem, const float4* sc, float f, int lo, int hi) {
   float top = -INFINITY;
+  uint32_t u[2][32];
+  tmem_ld32(s_tmem, u[0]);
+#pragma unroll 1
+  for (int c0 = 0; c0 < KT / 32; c0 += 2) {
 #pragma unroll
-  for (int c = 0; c < KT / 32; ++c)
+    for (int e = 0; e < 2; ++e) {
+      const int c = c0 + e;
+      tmem_wait_ld();
+      if (c + 1 < KT / 32) tmem_ld32(s_tmem + 32 * (c + 1), u[1 - e]);
+      mask_scores<EDGE>(u[e], 32 * c, lo, hi);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float a = __uint_as_float(u[c][16 * h]), b = __uint_as_float(u[c][16 * h + 1]);
+      for (int h = 0; h < 2; ++h) {
+        float a = __uint_as_float(u[e][16 * h]), b = __uint_as_float(u[e][16 * h + 1]);
 #pragma unroll
-      for (int j = 2; j < 14; j += 4) {
-        a = max3(a, __uint_as_float(u[c][16 * h + j]), __uint_as_float(u[c][16 * h + j + 1]));
-        b = max3(b, __uint_as_float(u[c][16 * h + j + 2]), __uint_as_float(u[c][16 * h + j + 3]));
+        for (int j = 2; j < 14; j += 4) {
+          a = max3(a, __uint_as_float(u[e][16 * h + j]), __uint_as_float(u[e][16 * h + j + 1]));
+          b = max3(b, __uint_as_float(u[e][16 * h + j + 2]), __uint_as_float(u[e][16 * h + j + 3]));
+        }
+        const float most = fmaxf(max3(a, __uint_as_float(u[e][16 * h + 14]), __uint_as_float(u[e][16 * h + 15])), b);
+        const float4 g = sc[2 * c + h];
+        const float t = fmaf(most, f * g.x, g.y);
+        top = fmaxf(top, EDGE && most == -INFINITY ? -INFINITY : t);
       }
-      const float most = fmaxf(max3(a, __uint_as_float(u[c][16 * h + 14]), __uint_as_float(u[c][16 * h + 15])), b);
-      const float4 g = sc[2 * c + h];
-      const float t = fmaf(most, f * g.x, g.y);
-      top = fmaxf(top, EDGE && most == -INFINITY ? -INFINITY : t);
     }
+  }
   return top;
 }
 // The weights of a tile, in f16 over its scores; returns what the sum of weights gains.
 template <bool EDGE, int KT>
-__device__ __forceinline__ float tile_weights(const uint32_t (&u)[KT / 32][32], uint32_t s_tmem, const float4* sc, float f, float from) {
+__device__ __forceinline__ float tile_weights(uint32_t s_tmem, const float4* sc, float f, float from, int lo, int hi) {
   float l = 0.0f;
+  uint32_t u[2][32];
+  tmem_ld32(s_tmem, u[0]);
+#pragma unroll 1
+  for (int c0 = 0; c0 < KT / 32; c0 += 2) {
 #pragma unroll
-  for (int c = 0; c < KT / 32; ++c) {
-    uint32_t w[16];
+    for (int e = 0; e < 2; ++e) {
+      const int c = c0 + e;
+      uint32_t w[16];
+      tmem_wait_ld();
+      if (c + 1 < KT / 32) tmem_ld32(s_tmem + 32 * (c + 1), u[1 - e]);
+      mask_scores<EDGE>(u[e], 32 * c, lo, hi);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float4 g = sc[2 * c + h];
-      const float by = f * g.x, add = g.y - from;
-      const uint64_t by2 = pack2(by, by), add_2 = pack2(add, add);
-      uint64_t sum2 = pack2(0.0f, 0.0f);
+      for (int h = 0; h < 2; ++h) {
+        const float4 g = sc[2 * c + h];
+        const float by = f * g.x, add = g.y - from;
+        const uint64_t by2 = pack2(by, by), add_2 = pack2(add, add);
+        uint64_t sum2 = pack2(0.0f, 0.0f);
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        const float u0 = __uint_as_float(u[c][16 * h + j]), u1 = __uint_as_float(u[c][16 * h + j + 1]);
-        float x0, x1;
-        unpack2(fma2(pack2(u0, u1), by2, add_2), x0, x1);
-        if constexpr (EDGE) {  // what a row does not see stays -inf, whatever the scale
-          x0 = u0 == -INFINITY ? u0 : x0;
-          x1 = u1 == -INFINITY ? u1 : x1;
+        for (int j = 0; j < 16; j += 2) {
+          const float u0 = __uint_as_float(u[e][16 * h + j]), u1 = __uint_as_float(u[e][16 * h + j + 1]);
+          float x0, x1;
+          unpack2(fma2(pack2(u0, u1), by2, add_2), x0, x1);
+          if constexpr (EDGE) {  // what a row does not see stays -inf, whatever the scale
+            x0 = u0 == -INFINITY ? u0 : x0;
+            x1 = u1 == -INFINITY ? u1 : x1;
+          }
+          x0 = exp2_fast(x0), x1 = exp2_fast(x1);
+          sum2 = add2(sum2, pack2(x0, x1));
+          const __half2 x = __floats2half2_rn(x0, x1);
+          w[8 * h + j / 2] = *reinterpret_cast<const uint32_t*>(&x);
         }
-        x0 = exp2_fast(x0), x1 = exp2_fast(x1);
-        sum2 = add2(sum2, pack2(x0, x1));
-        const __half2 x = __floats2half2_rn(x0, x1);
-        w[8 * h + j / 2] = *reinterpret_cast<const uint32_t*>(&x);
+        float a, b;
+        unpack2(sum2, a, b);
+        // a row that sees nothing of a page whose scale is not a number: nothing, and not 0 x NaN
+        l = EDGE && a + b == 0.0f ? l : fmaf(a + b, g.z, l);
       }
-      float a, b;
-      unpack2(sum2, a, b);
-      // a row that sees nothing of a page whose scale is not a number: nothing, and not 0 x NaN
-      l = EDGE && a + b == 0.0f ? l : fmaf(a + b, g.z, l);
+      tmem_st16(s_tmem + 16 * c, w);
     }
-    tmem_st16(s_tmem + 16 * c, w);
   }
   return l;
 }
@@ -596,6 +620,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       proxy_fence();
       warp_arrive(q_full + 8 * rt);
     };
+    auto prefetch = [&]() {  // the same row into L2, a tile's time and more ahead
+      const int q = min(next.row_block + rt * kRowTile + row, next.row_block + next.rows - 1), bytes = A.q_dtype == LX_BF16 ? 2 : 4;
+      const uint8_t* src = static_cast<const uint8_t*>(A.q) +
+                           ((next.q.row0 + q / A.group) * A.ld_q + (static_cast<int64_t>(next.head) * A.group + q % A.group) * D) * bytes;
+      for (int b = 0; b < D * bytes; b += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + b));
+    };
     auto takes = [&](const Part& x) { return rt < RT && (rt == 0 || x.rows > kRowTile); };
     if (more_parts && takes(next)) queries();
     while (ok && more_parts) {
@@ -625,17 +655,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         tc_fence_after();
         const bool edge = key0 + KT > past_low || key0 < see_all;
         const int lo = low - key0, hi = past - key0;
-        uint32_t u[KT / 32][32];
-#pragma unroll
-        for (int c = 0; c < KT / 32; ++c) tmem_ld32(s_tmem + 32 * c, u[c]);
-        tmem_wait_ld();
-        float top;
-        if (edge) {
-          mask_scores<true, KT>(u, lo, hi);
-          top = tile_top<true, KT>(u, sc, f_now);
-        } else {
-          top = tile_top<false, KT>(u, sc, f_now);
-        }
+        const float top = edge ? tile_top<true, KT>(s_tmem, sc, f_now, lo, hi) : tile_top<false, KT>(s_tmem, sc, f_now, lo, hi);
         const bool higher = top > m + kSlack;  // at first m is -inf
         if (__any_sync(0xffffffffu, higher)) {
           const float shrink = higher ? exp2_fast(m - top) : 1.0f;
@@ -655,11 +675,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           }
         }
         const float from = (m == -INFINITY ? 0.0f : m) - kShift;
-        l += edge ? tile_weights<true, KT>(u, s_tmem, sc, f_now, from) : tile_weights<false, KT>(u, s_tmem, sc, f_now, from);
+        l += edge ? tile_weights<true, KT>(s_tmem, sc, f_now, from, lo, hi) : tile_weights<false, KT>(s_tmem, sc, f_now, from, lo, hi);
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(p_full + 8 * rt);
-        if (i == 0) more_parts = next_part<C::kRows>(T, share, next);
+        if (i == 0) {
+          more_parts = next_part<C::kRows>(T, share, next);
+          if (more_parts && takes(next)) prefetch();
+        }
       }
       tiles_done += p.tiles;
       if (!ok) break;
@@ -686,15 +709,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           tmem_wait_ld();
           if (valid) {
 #pragma unroll
-            for (int q = 0; q < 16; q += 2) {
+            for (int q = 0; q < 16; q += 4) {
               const int d = 4 * (W * h + 16 * k + q);
-              const float4 a = make_float4(__uint_as_float(u[0][q]), __uint_as_float(u[1][q]), __uint_as_float(u[2][q]), __uint_as_float(u[3][q]));
-              const float4 b = make_float4(__uint_as_float(u[0][q + 1]), __uint_as_float(u[1][q + 1]), __uint_as_float(u[2][q + 1]), __uint_as_float(u[3][q + 1]));
+              float v[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(u[e & 3][q + e / 4]);
               if (p.whole) {
-                store_out8(A, out_row + d, a, b, factor, T.out_vec8);
+                store_out16(A, out_row + d, v, factor, T.out_whole);
               } else {
-                *reinterpret_cast<float4*>(part + 2 * C::kRows + pr * D + d) = a;
-                *reinterpret_cast<float4*>(part + 2 * C::kRows + pr * D + d + 4) = b;
+                uint32_t w[8];
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(v[8 * z + e]);
+                  store8(part + 2 * C::kRows + pr * D + d + 8 * z, w);
+                }
               }
             }
           }
@@ -717,70 +746,90 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         const uint8_t* const raw_v = raw_k + RS * C::kRawBytes;
         auto seen = [&](int j) { return all || (slot0 + j < p.past_high && slot0 + j >= p.see_low); };
         // keys. Lane i of eight takes key i of a run, and of its pieces of 16 bytes another one than its neighbours: neither the reads of
-        // rows nor the writes of core matrices meet in a bank
-        if (!warp_wait(raw_full + 8 * (n % RS), n / RS & 1, V.status) || !warp_wait(k_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
+        // rows nor the writes of core matrices meet in a bank. The codes are taken into registers first, so that the next ones come
+        // while these are widened.
+        if (!warp_wait(raw_full + 8 * (n % RS), n / RS & 1, V.status)) {
           ok = false;
           break;
         }
         {
-          constexpr int PIECES = D / 16;
-          const uint32_t dst = k_base + n % NS * C::kKvBytes;
+          constexpr int PIECES = D / 16, RUNS = WK / 8;
           const int key8 = lane & 7;
-#pragma unroll 1
-          for (int a = 0; a < WK / 8; ++a) {
+          auto piece_at = [&](int b) { return ((D == 64 ? key8 >> 1 : key8) + 4 * b + (lane >> 3)) & (PIECES - 1); };
+          uint4 x[RUNS][PIECES / 4];
+#pragma unroll
+          for (int a = 0; a < RUNS; ++a) {
             const int key = w4 * WK + 8 * a + key8;
             const bool use = seen(key) && scales[n % C::kScaleRing * C::kScaleGroups + key / 16].w != 0.0f;
 #pragma unroll
             for (int b = 0; b < PIECES / 4; ++b) {
-              const int piece = ((D == 64 ? key8 >> 1 : key8) + 4 * b + (lane >> 3)) & (PIECES - 1);
-              uint4 x = *reinterpret_cast<const uint4*>(raw_k + key * D + 16 * piece);
-              if (!use) x = make_uint4(0, 0, 0, 0);
-              const uint32_t word[4] = {x.x, x.y, x.z, x.w};
+              x[a][b] = *reinterpret_cast<const uint4*>(raw_k + key * D + 16 * piece_at(b));
+              if (!use) x[a][b] = make_uint4(0, 0, 0, 0);
+            }
+          }
+          warp_arrive(raw_empty + 8 * (n % RS));
+          if (!warp_wait(k_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = k_base + n % NS * C::kKvBytes;
+#pragma unroll
+          for (int a = 0; a < RUNS; ++a)
+#pragma unroll
+            for (int b = 0; b < PIECES / 4; ++b) {
+              const uint32_t word[4] = {x[a][b].x, x[a][b].y, x[a][b].z, x[a][b].w};
               uint32_t o[8];
 #pragma unroll
               for (int c = 0; c < 4; ++c) halves<kInt8>(word[c], o[2 * c], o[2 * c + 1]);
-              const uint32_t to = dst + 2 * piece * (KT * 16) + key * 16;
+              const uint32_t to = dst + 2 * piece_at(b) * (KT * 16) + (w4 * WK + 8 * a + key8) * 16;
               sts128(to, o[0], o[1], o[2], o[3]);
               sts128(to + KT * 16, o[4], o[5], o[6], o[7]);
             }
-          }
         }
-        warp_arrive(raw_empty + 8 * (n % RS));
         proxy_fence();
         warp_arrive(k_full + 8 * (n % NS));
         // values: lane: four dims of eight keys; with 64 values per head the half warps have a run of eight keys each
-        if (!warp_wait(raw_full + 8 * (RS + n % RS), n / RS & 1, V.status) || !warp_wait(v_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
+        if (!warp_wait(raw_full + 8 * (RS + n % RS), n / RS & 1, V.status)) {
           ok = false;
           break;
         }
         {
           constexpr int LANES = D < 128 ? D / 4 : 32, AT_ONCE = 32 / LANES, RUNS = WK / (8 * AT_ONCE), HALVES = D > 128 ? 2 : 1;
           const int l = lane % LANES, sub = lane / LANES;
-          const uint32_t dst = v_base + n % NS * C::kKvBytes;
-#pragma unroll 1
+          uint32_t x[RUNS][HALVES][8];
+#pragma unroll
           for (int a = 0; a < RUNS; ++a) {
             const int run = w4 * (WK / 8) + a * AT_ONCE + sub;
             const bool use = scales[n % C::kScaleRing * C::kScaleGroups + run / 2].w != 0.0f;
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h) {
-              uint32_t x[8], o[4][4];  // o: dim, pair of keys
+            for (int h = 0; h < HALVES; ++h)
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                x[j] = *reinterpret_cast<const uint32_t*>(raw_v + (8 * run + j) * D + 128 * h + 4 * l);
-                if (!use || !seen(8 * run + j)) x[j] = 0;
+                x[a][h][j] = *reinterpret_cast<const uint32_t*>(raw_v + (8 * run + j) * D + 128 * h + 4 * l);
+                if (!use || !seen(8 * run + j)) x[a][h][j] = 0;
               }
+          }
+          warp_arrive(raw_empty + 8 * (RS + n % RS));
+          if (!warp_wait(v_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = v_base + n % NS * C::kKvBytes;
+#pragma unroll
+          for (int a = 0; a < RUNS; ++a)
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) {
+              uint32_t o[4][4];  // dim, pair of keys
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                halves<kInt8>(__byte_perm(x[2 * j], x[2 * j + 1], 0x5140), o[0][j], o[1][j]);
-                halves<kInt8>(__byte_perm(x[2 * j], x[2 * j + 1], 0x7362), o[2][j], o[3][j]);
+                halves<kInt8>(__byte_perm(x[a][h][2 * j], x[a][h][2 * j + 1], 0x5140), o[0][j], o[1][j]);
+                halves<kInt8>(__byte_perm(x[a][h][2 * j], x[a][h][2 * j + 1], 0x7362), o[2][j], o[3][j]);
               }
-              const uint32_t to = dst + run * (D * 16) + (128 * h + l) * 16;
+              const uint32_t to = dst + (w4 * (WK / 8) + a * AT_ONCE + sub) * (D * 16) + (128 * h + l) * 16;
 #pragma unroll
               for (int d = 0; d < 4; ++d) sts128(to + d * LANES * 16, o[d][0], o[d][1], o[d][2], o[d][3]);
             }
-          }
         }
-        warp_arrive(raw_empty + 8 * (RS + n % RS));
         proxy_fence();
         warp_arrive(v_full + 8 * (n % NS));
       }
@@ -869,7 +918,7 @@ int tile_attention(AttentionArgs A, int head_dim, bool int8, int limit, void* wo
   T.a.min_tiles = 2 * kBlockCost + 2;
   T.header = reinterpret_cast<PlanHeader*>(ws), T.plan = reinterpret_cast<BlockPlan*>(ws + L.plan), T.partial = reinterpret_cast<float*>(ws + L.partial);
   T.capacity = L.capacity;
-  T.out_vec8 = aligned(A.out, 16) && A.ld_out % 8 == 0;
+  T.out_whole = aligned(A.out, 32) && A.ld_out % 16 == 0;
   T.q_vec = aligned(A.q, 16) && A.ld_q % (A.q_dtype == LX_BF16 ? 8 : 4) == 0;
   switch (head_dim) {
     case 64: return int8 ? launch_tile<true, 64>(T, stream) : launch_tile<false, 64>(T, stream);

@@ -334,7 +334,7 @@ LX_API int lx_b200_kv_append(const lx_b200_kv_cache* cache, const lx_b200_kv_bat
  * head h / (q_heads / kv_heads) of the slots j <= p, with window > 0 of the last `window` of these (itself counted), and
  * out = sum_j softmax_j(scale * q . k_j) v_j. q: rows of q_heads * head_dim, f32 or bf16; out the same in bf16; a query that sees no slot
  * gets zeros. What unused slots and the table past a sequence's end hold is not read into any result; a page outside the
- * cache makes the rows that see it NaN. f32 sums and statistics. workspace: lx_b200_attention_workspace_bytes, 16-byte aligned,
+ * cache makes the rows that see it NaN. f32 sums and statistics. workspace: lx_b200_attention_workspace_bytes, 256-byte aligned,
  * what it holds does not matter; calls that may overlap need one each. A row's bits depend on the batch it is in (the keys of
  * a sequence are cut to even out the work) and are the same every time. */
 LX_API int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q,

@@ -84,7 +84,7 @@ def test_appends_that_are_refused(lib):
 
 
 def test_attentions_that_are_refused(lib):
-    for kw in (dict(q=None), dict(out=None), dict(ld_q=255), dict(ld_out=255), dict(q_dtype=2), dict(q_heads=0), dict(q_heads=5), dict(window=-1), dict(workspace=None), dict(workspace=4104)):
+    for kw in (dict(q=None), dict(out=None), dict(ld_q=255), dict(ld_out=255), dict(q_dtype=2), dict(q_heads=0), dict(q_heads=5), dict(window=-1), dict(workspace=None), dict(workspace=4096 + 128)):
         assert attend(lib, cache(), batch(tokens=4), **kw) == abi.ERR_INVALID, kw
     assert lib.lx_b200_attention_workspace_bytes(address(cache()), address(batch()), 4) >= 0
     for args in ((None, batch(), 4), (cache(), None, 4), (cache(), batch(), 5), (cache(), batch(), 0), (cache(), batch(max_new=-1), 4), (cache(head_dim=80), batch(), 4)):
