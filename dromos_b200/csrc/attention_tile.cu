@@ -1,8 +1,9 @@
 // Attention of many query rows per key head (prompts, pieces of prompts, groups of drafted tokens): both products on tcgen05.
 //
 // The mathematics is that of attention.cu: codes widened exactly to f16, scales outside in f32, t_j = c kscale (q . kcode_j) + log2 vscale,
-// weights 2^(12 + t_j - m) that go to the second product in f16. m is a maximum the row had earlier: it moves when a larger one is more
-// than 3 above it (2^15 is inside f16's range), which spares the accumulator nearly every rescaling.
+// weights 2^(7 + t_j - m) that go to the second product in f16. m is a maximum the row had earlier: it moves when a larger one is more
+// than 8 above it (2^15 is inside f16's range; a weight's smallest step, 2^-24, is 2^-31 of the largest weight or less), which spares
+// the accumulator nearly every rescaling.
 //
 // A CTA takes 256 rows (128 where a head has 256 values) of one sequence and key head, a row being a new token and one of the heads that
 // share the keys, in two tiles of 128: S = Q K^T of one tile runs while the other's softmax does. Roles: two groups of four warps each
@@ -26,11 +27,11 @@ constexpr int kSoftmaxWarps = 8, kWidenWarps = 4;
 constexpr int kMmaWarp = kSoftmaxWarps + kWidenWarps, kLoadWarp = kMmaWarp + 1;
 constexpr int kTileThreads = 32 * (kMmaWarp + 4);  // whole groups of four warps, each with its own share of the registers
 // Registers a thread: 128 at launch (512 threads), 65,536 in all; 256 x kSoftmaxRegs + 128 x kWidenRegs + 128 x kMmaRegs are as many.
-constexpr int kSoftmaxRegs = 160, kWidenRegs = 96, kMmaRegs = 96;
+constexpr int kSoftmaxRegs = 176, kWidenRegs = 80, kMmaRegs = 80;
 static_assert(256 * kSoftmaxRegs + 128 * kWidenRegs + 128 * kMmaRegs <= 512 * 128, "more registers than the launch has");
-constexpr int kBlockCost = 4;
-constexpr int kShift = 12;  // the largest weights are 2^12 .. 2^15
-constexpr float kSlack = 3.0f, kUnshift = 0x1p-12f;
+constexpr int kBlockCost = 6;
+constexpr int kShift = 7;  // the largest weights are 2^7 .. 2^15
+constexpr float kSlack = 8.0f, kUnshift = 0x1p-7f;
 
 template <int D>
 struct TileCfg {
@@ -741,10 +742,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     while (ok && next_part<C::kRows>(T, share, p)) {
       for (int i = 0; i < p.tiles && ok; ++i, ++n) {
         const int slot0 = (p.tile + i) * KT;
-        const bool all = slot0 >= p.see_low && slot0 + KT <= p.past_high;  // else what no row sees, which was not copied, reads as 0
         const uint8_t* const raw_k = smem + C::kRawOff + n % RS * C::kRawBytes;
         const uint8_t* const raw_v = raw_k + RS * C::kRawBytes;
-        auto seen = [&](int j) { return all || (slot0 + j < p.past_high && slot0 + j >= p.see_low); };
+        // a word of slot j: all of it, or 0 where no row sees the slot (what it holds may be no numbers) or nothing was copied
+        const float4* const sc = scales + n % C::kScaleRing * C::kScaleGroups;
+        auto keep = [&](int j) {
+          const bool there = slot0 + j < p.past_high && slot0 + j >= p.see_low && sc[j / 16].w != 0.0f;
+          return there ? 0xffffffffu : 0u;
+        };
         // keys. Lane i of eight takes key i of a run, and of its pieces of 16 bytes another one than its neighbours: neither the reads of
         // rows nor the writes of core matrices meet in a bank. The codes are taken into registers first, so that the next ones come
         // while these are widened.
@@ -752,19 +757,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           ok = false;
           break;
         }
+        bool edge = slot0 < p.see_low || slot0 + KT > p.past_high;
+#pragma unroll
+        for (int g = 0; g < C::kScaleGroups; ++g) edge |= sc[g].w == 0.0f;
         {
           constexpr int PIECES = D / 16, RUNS = WK / 8;
           const int key8 = lane & 7;
           auto piece_at = [&](int b) { return ((D == 64 ? key8 >> 1 : key8) + 4 * b + (lane >> 3)) & (PIECES - 1); };
           uint4 x[RUNS][PIECES / 4];
 #pragma unroll
-          for (int a = 0; a < RUNS; ++a) {
-            const int key = w4 * WK + 8 * a + key8;
-            const bool use = seen(key) && scales[n % C::kScaleRing * C::kScaleGroups + key / 16].w != 0.0f;
+          for (int a = 0; a < RUNS; ++a)
 #pragma unroll
-            for (int b = 0; b < PIECES / 4; ++b) {
-              x[a][b] = *reinterpret_cast<const uint4*>(raw_k + key * D + 16 * piece_at(b));
-              if (!use) x[a][b] = make_uint4(0, 0, 0, 0);
+            for (int b = 0; b < PIECES / 4; ++b) x[a][b] = *reinterpret_cast<const uint4*>(raw_k + (w4 * WK + 8 * a + key8) * D + 16 * piece_at(b));
+          if (edge) {
+#pragma unroll
+            for (int a = 0; a < RUNS; ++a) {
+              const uint32_t k = keep(w4 * WK + 8 * a + key8);
+#pragma unroll
+              for (int b = 0; b < PIECES / 4; ++b) x[a][b] = make_uint4(x[a][b].x & k, x[a][b].y & k, x[a][b].z & k, x[a][b].w & k);
             }
           }
           warp_arrive(raw_empty + 8 * (n % RS));
@@ -800,13 +810,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
 #pragma unroll
           for (int a = 0; a < RUNS; ++a) {
             const int run = w4 * (WK / 8) + a * AT_ONCE + sub;
-            const bool use = scales[n % C::kScaleRing * C::kScaleGroups + run / 2].w != 0.0f;
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
 #pragma unroll
+              for (int j = 0; j < 8; ++j) x[a][h][j] = *reinterpret_cast<const uint32_t*>(raw_v + (8 * run + j) * D + 128 * h + 4 * l);
+          }
+          if (edge) {
+#pragma unroll
+            for (int a = 0; a < RUNS; ++a)
+#pragma unroll
               for (int j = 0; j < 8; ++j) {
-                x[a][h][j] = *reinterpret_cast<const uint32_t*>(raw_v + (8 * run + j) * D + 128 * h + 4 * l);
-                if (!use || !seen(8 * run + j)) x[a][h][j] = 0;
+                const uint32_t k = keep(8 * (w4 * (WK / 8) + a * AT_ONCE + sub) + j);
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) x[a][h][j] &= k;
               }
           }
           warp_arrive(raw_empty + 8 * (RS + n % RS));

@@ -7,10 +7,10 @@ Tolerances, derived from the roundings of each operator:
              angle's rounding to f32, 2^-24 * pi), so its code may be that of a value so far off.
   queries    the same 2^-21, and their rounding to bf16, 2^-8 of the value (f32: none).
   attention  the rounding of the result to bf16, 2^-8 |o|; the weights' rounding to f16, 2^-11 of sum w |v|, and as much again for f32
-             sums and exponentials; weights are scaled so that the largest w v-scale is 2^12 or more, so those below f16's normal
-             range are off by 2^-37 of it at most (half of 2^-24); with codes of up to 448 (or 127) whose largest is at least half of that
-             in every page a key adds 2^-37 max(w v-scale top), and max(w v-scale top) <= 2 max over the dims of sum w |v|:
-             n 2^-36 of that in all; scores that are off by d move every weight by a factor within
+             sums and exponentials; weights are scaled so that the largest w v-scale is 2^7 or more, so those below f16's normal
+             range are off by 2^-32 of it at most (half of 2^-24); with codes of up to 448 (or 127) whose largest is at least half of that
+             in every page a key adds 2^-32 max(w v-scale top), and max(w v-scale top) <= 2 max over the dims of sum w |v|:
+             n 2^-31 of that in all; scores that are off by d move every weight by a factor within
              1 +- 2 d: d = |scale| sum |q k| (2^-11 for queries in f32, which are rounded to f16; D 2^-24 for the sum).
   norm       mean squares of positive terms 2^-19 (at most 32 + 10 additions in a chain, 2^-24 each), halved by the root; some
              more factors of 2^-24: 2^-19 of a term in all; bf16 results 2^-8 more.
@@ -220,7 +220,7 @@ def check_attention(lx, S, K, G, D, kind, window=0, dtype=torch.bfloat16, seed=0
         at = slice(h * D, (h + 1) * D)
         d[:, at] = (abs(attend.scale) * (qd[:, at].abs() * kmax[h // G]).sum(1, keepdim=True) * unit)
     bound = (want.abs() * 2.0**-8 + size * (2.0**-10 + 2 * d))[:S.tokens] + 1e-30
-    bound += (size.reshape(S.rows, H, D).amax(2, keepdim=True) * 2.0**-36 * max(S.total)).expand(-1, -1, D).reshape(S.rows, -1)[:S.tokens]
+    bound += (size.reshape(S.rows, H, D).amax(2, keepdim=True) * 2.0**-31 * max(S.total)).expand(-1, -1, D).reshape(S.rows, -1)[:S.tokens]
     far = (o - want[:S.tokens]).abs() / bound
     assert float(far.max()) <= 1.0, f"{float(far.max()):.2f} times the bound"
 
