@@ -14,6 +14,7 @@ namespace b200 {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kJoinThreads = 256;
 constexpr int kTile = 16 * kWarps;  // slots of a tile: 16 for each warp
 
 // Work of a sequence: units (blocks of ROWS query rows x key heads) of equally many tiles.
@@ -36,7 +37,7 @@ __device__ __forceinline__ SeqWork work_of(const AttentionArgs& A, int s) {
   return w;
 }
 
-// Every CTA has the same count of consecutive tiles of the whole batch, `per`; a unit that several CTAs share is joined by join_kernel.
+// Every CTA has the same count of consecutive tiles of the whole batch, `per`; a unit that several CTAs share is joined by a second kernel.
 // Called by all threads; `sums`: shared. The sequence that holds tile `at` and its first tile's number come back in shared memory.
 struct Place {
   int64_t total, base;  // base: tiles of the sequences before `seq`
@@ -143,11 +144,16 @@ __global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3
   __shared__ Place place;
   __shared__ int64_t sums[kWarps];
   pdl_wait();
+  pdl_trigger();  // the join waits for the whole of this kernel; it may be brought up before
   const KvView& C = A.kv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   int64_t per, at;
   const Place start = find_tile<ROWS>(A, blockIdx.x, gridDim.x, per, at, &place, sums);
-  if (start.seq < 0) return;
+  JoinInfo join{};
+  if (start.seq < 0) {
+    if (tid == 0) A.join[blockIdx.x] = join;
+    return;
+  }
   const int64_t end = min(start.total, at + per);
   int s = start.seq;
   int64_t base = start.base;
@@ -391,42 +397,70 @@ __global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3
     }
     __syncthreads();  // before the next unit's queries and sums
     at = unit_at + part1;
+    if (part0 == 0 && !complete) join = {W.q.row0, row_block, rows, head, static_cast<int>((unit_at + W.tiles - 1) / per), {}};
   }
+  if (tid == 0) A.join[blockIdx.x] = join;
 }
 
-// Joins the units that several CTAs of the stream kernel shared: CTA i the one that began in piece i and went on into the next.
+// Joins the units that several CTAs of the stream kernel shared: CTA i the one that began in share i and went on into the next. The
+// parts' maxima and sums are looked at 32 parts at once, then their accumulators are read without one waiting for the other (a loop
+// that carried the maximum from part to part took decode of one sequence of 4099 tokens from 17 us to what the parts cost).
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ AttentionArgs A) {
-  constexpr int ROWS = 8 * NT;
-  __shared__ Place place;
-  __shared__ int64_t sums[kWarps];
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttentionArgs A) {
+  constexpr int ROWS = 8 * NT, AT_ONCE = 32, ITEMS = (ROWS * (D / 4) + kJoinThreads - 1) / kJoinThreads;
+  __shared__ float ms[AT_ONCE][ROWS], ls[AT_ONCE][ROWS], shrink[ROWS], sums[ROWS], tops[ROWS];
   pdl_wait();
-  int64_t per, at;
-  const int pieces = gridDim.x;
-  const Place here = find_tile<ROWS>(A, blockIdx.x + 1, pieces, per, at, &place, sums);
-  if (here.seq < 0) return;
-  const SeqWork W = work_of<ROWS>(A, here.seq);
-  const int unit = static_cast<int>((at - here.base) / W.tiles);
-  const int64_t u0 = here.base + static_cast<int64_t>(unit) * W.tiles, u1 = u0 + W.tiles;
-  if (u0 == at || u0 < at - per) return;  // nothing crosses this border, or it began earlier
-  const int last = static_cast<int>((u1 - 1) / per);
-  const int head = unit % A.kv.kv_heads, row_block = unit / A.kv.kv_heads * ROWS, rows = min(ROWS, W.q.n * A.group - row_block);
+  const JoinInfo u = A.join[blockIdx.x];
+  if (u.rows == 0) return;
+  const int tid = threadIdx.x, first = blockIdx.x;
   const int64_t slot_floats = ROWS * (D + 2);
-  for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4;
-    float top = -INFINITY, sum = 0.0f;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p = blockIdx.x; p <= last; ++p) {
-      const float* src = A.partial + (2 * static_cast<int64_t>(p) + (p == static_cast<int>(blockIdx.x))) * slot_floats;
-      const float mp = src[r], lp = src[ROWS + r], next = fmaxf(top, mp);
-      const float4 op = *reinterpret_cast<const float4*>(src + 2 * ROWS + r * D + d);
-      const float a = top == -INFINITY ? 0.0f : exp2_fast(top - next), b = mp == -INFINITY ? 0.0f : exp2_fast(mp - next);
-      sum = (top == -INFINITY ? sum : sum * a) + (mp == -INFINITY ? lp : lp * b);
-      v.x = v.x * a + op.x * b, v.y = v.y * a + op.y * b, v.z = v.z * a + op.z * b, v.w = v.w * a + op.w * b;
-      top = next;
+  auto slot = [&](int p) { return A.partial + (2 * static_cast<int64_t>(p) + (p == first)) * slot_floats; };
+  if (tid < ROWS) sums[tid] = 0.0f, tops[tid] = -INFINITY;
+  float4 v[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int p0 = first; p0 <= u.last; p0 += AT_ONCE) {
+    const int n = min(AT_ONCE, u.last + 1 - p0);
+    __syncthreads();
+    for (int i = tid; i < n * ROWS; i += kJoinThreads) {
+      const float* src = slot(p0 + i / ROWS) + i % ROWS;
+      if (i % ROWS < u.rows) ms[i / ROWS][i % ROWS] = src[0], ls[i / ROWS][i % ROWS] = src[ROWS];
     }
-    const int token = (row_block + r) / A.group, qh = head * A.group + (row_block + r) % A.group;
-    store_out(A, (W.q.row0 + token) * A.ld_out + static_cast<int64_t>(qh) * D + d, v, sum == 0.0f ? 0.0f : 0x1p-14f / sum);
+    __syncthreads();
+    if (tid < u.rows) {
+      float top = tops[tid], sum = sums[tid];
+      for (int p = 0; p < n; ++p) top = fmaxf(top, ms[p][tid]);
+      shrink[tid] = tops[tid] == -INFINITY ? 0.0f : exp2_fast(tops[tid] - top);
+      // a part whose scores were all not-a-number has no maximum, its sums say so
+      sum = tops[tid] == -INFINITY ? sum : sum * shrink[tid];
+      for (int p = 0; p < n; ++p) {
+        const float m = ms[p][tid], k = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+        sum += m == -INFINITY ? ls[p][tid] : ls[p][tid] * k;
+        ms[p][tid] = k;
+      }
+      tops[tid] = top, sums[tid] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int at = tid + i * kJoinThreads, r = at / (D / 4), d = at % (D / 4) * 4;
+      if (r >= u.rows) continue;
+      const float k0 = shrink[r];
+      v[i] = make_float4(v[i].x * k0, v[i].y * k0, v[i].z * k0, v[i].w * k0);
+#pragma unroll 8
+      for (int p = 0; p < n; ++p) {
+        const float4 o = *reinterpret_cast<const float4*>(slot(p0 + p) + 2 * ROWS + r * D + d);
+        const float k = ms[p][r];
+        v[i].x = fmaf(o.x, k, v[i].x), v[i].y = fmaf(o.y, k, v[i].y), v[i].z = fmaf(o.z, k, v[i].z), v[i].w = fmaf(o.w, k, v[i].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int at = tid + i * kJoinThreads, r = at / (D / 4), d = at % (D / 4) * 4;
+    if (r >= u.rows) continue;
+    const int token = (u.row_block + r) / A.group, qh = u.head * A.group + (u.row_block + r) % A.group;
+    store_out(A, (u.row0 + token) * A.ld_out + static_cast<int64_t>(qh) * D + d, v[i], sums[r] == 0.0f ? 0.0f : 0x1p-14f / sums[r]);
   }
 }
 
@@ -440,16 +474,17 @@ constexpr size_t stream_smem() {
 }
 template <int D, int NT>
 int64_t stream_workspace() {
-  return static_cast<int64_t>(sm_count()) * stream_ctas<D, NT>() * 2 * 8 * NT * (D + 2) * 4;
+  return static_cast<int64_t>(sm_count()) * stream_ctas<D, NT>() * (2 * 8 * NT * (D + 2) * 4 + static_cast<int64_t>(sizeof(JoinInfo)));
 }
 template <bool kInt8, int D, int NT>
-int launch_stream_attention(const AttentionArgs& A, cudaStream_t stream) {
+int launch_stream_attention(AttentionArgs A, cudaStream_t stream) {
   const unsigned grid = static_cast<unsigned>(sm_count()) * stream_ctas<D, NT>();
   if (grid == 0) return kNotSupported;
+  A.join = reinterpret_cast<JoinInfo*>(A.partial + static_cast<int64_t>(grid) * 2 * 8 * NT * (D + 2));
   auto kernel = attention_stream_kernel<kInt8, D, NT>;
   if (int e = allow_dynamic_smem<(kInt8 * 4 + (D == 64 ? 0 : D == 128 ? 1 : 2)) * 8 + NT>(kernel)) return e;
   if (int e = launch_kernel(kernel, dim3(grid), dim3(kThreads), stream_smem<D, NT>(), stream, A)) return e;
-  return launch_kernel(attention_join_kernel<D, NT>, dim3(grid), dim3(kThreads), 0, stream, A);
+  return launch_kernel(attention_join_kernel<D, NT>, dim3(grid), dim3(kJoinThreads), 0, stream, A);
 }
 // Groups of 8 rows that a CTA of the stream kernel takes at once: as few as hold a sequence's rows, 4 at most (2 with 256 values per
 // head), whose accumulators fill the registers.

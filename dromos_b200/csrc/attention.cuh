@@ -6,11 +6,17 @@
 
 namespace b200 {
 
+// What a CTA of the stream kernel leaves for the join: the unit that begins in its share and goes on into the next one's, rows 0 where there is none.
+struct JoinInfo {
+  int row0, row_block, rows, head, last, pad[3];  // last: the share that holds the unit's end
+};
+
 struct AttentionArgs {
   KvView kv;
   const void* q;
   uint16_t* out;
   float* partial;
+  JoinInfo* join;
   int64_t ld_q, ld_out;
   int q_dtype, q_heads, group, window, min_tiles;
   float scale_log2;  // the softmax's scale times log2 e

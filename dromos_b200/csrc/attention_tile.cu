@@ -876,16 +876,19 @@ __global__ void __launch_bounds__(256) attention_tile_join_kernel(const __grid_c
   const int rows = min(C::kRows, q.n * A.group - b.row_block);
   for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * (D / 4); i += gridDim.y * 256) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
+    auto slot = [&](int p) { return T.partial + (2 * static_cast<int64_t>(p) + (p == static_cast<int>(blockIdx.x))) * (C::kRows * (D + 2)); };
     float top = -INFINITY, sum = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int p = blockIdx.x; p <= last; ++p) top = fmaxf(top, slot(p)[r]);
+#pragma unroll 8
     for (int p = blockIdx.x; p <= last; ++p) {
-      const float* src = T.partial + (2 * static_cast<int64_t>(p) + (p == static_cast<int>(blockIdx.x))) * (C::kRows * (D + 2));
-      const float mp = src[r], lp = src[C::kRows + r], next = fmaxf(top, mp);
+      const float* src = slot(p);
+      const float mp = src[r], lp = src[C::kRows + r];
       const float4 op = *reinterpret_cast<const float4*>(src + 2 * C::kRows + r * D + d);
-      const float x = top == -INFINITY ? 0.0f : exp2_fast(top - next), y = mp == -INFINITY ? 0.0f : exp2_fast(mp - next);
-      sum = (top == -INFINITY ? sum : sum * x) + (mp == -INFINITY ? lp : lp * y);
-      v.x = v.x * x + op.x * y, v.y = v.y * x + op.y * y, v.z = v.z * x + op.z * y, v.w = v.w * x + op.w * y;
-      top = next;
+      const float y = mp == -INFINITY ? 0.0f : exp2_fast(mp - top);
+      sum += mp == -INFINITY ? lp : lp * y;
+      v.x = fmaf(op.x, y, v.x), v.y = fmaf(op.y, y, v.y), v.z = fmaf(op.z, y, v.z), v.w = fmaf(op.w, y, v.w);
     }
     const int rr = b.row_block + r;
     store_out(A, (q.row0 + rr / A.group) * A.ld_out + (static_cast<int64_t>(head) * A.group + rr % A.group) * D + d, v, sum == 0.0f ? 0.0f : kUnshift / sum);

@@ -222,29 +222,37 @@ class Experts:
         return out
 
 
+_DTYPES = {torch.bfloat16: abi.BF16, torch.float32: abi.F32}
+
+
 def _dtype(x: torch.Tensor, what: str) -> int:
-    if x.dtype == torch.bfloat16:
-        return abi.BF16
-    if x.dtype == torch.float32:
-        return abi.F32
-    raise TypeError(f"{what}: bfloat16 or float32, not {x.dtype}")
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise TypeError(f"{what}: bfloat16 or float32, not {x.dtype}")
+    return dt
 
 
-def _rows(x: torch.Tensor, rows: int, cols: int, what: str, device=None) -> int:
-    """The row stride of a [rows, cols] tensor whose rows are contiguous."""
-    if x.dim() != 2 or x.shape[0] != rows or x.shape[1] != cols or (cols > 1 and x.stride(1) != 1):
-        raise ValueError(f"{what}: [{rows}, {cols}] with contiguous rows, not {tuple(x.shape)} with strides {x.stride()}")
-    if device is not None and x.device != device:
+def _rows(x: torch.Tensor, rows: int, cols: int, what: str, device) -> int:
+    """The row stride of a [rows, cols] tensor on the device whose rows are contiguous."""
+    stride = x.stride()
+    if x.shape != (rows, cols) or (stride[1] != 1 and cols > 1):
+        raise ValueError(f"{what}: [{rows}, {cols}] with contiguous rows, not {tuple(x.shape)} with strides {stride}")
+    if x.device != device:
         raise ValueError(f"{what} is on {x.device}, the call on {device}")
-    return x.stride(0) if rows > 1 else max(cols, x.stride(0))
+    return stride[0] if rows > 1 else max(cols, stride[0])
 
 
-def _here(device: torch.device):
-    """Calls launch on the current device's current stream: a buffer of another device is refused, not touched."""
+_current_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device  # the first is the second without 1 us of checks
+
+
+def _stream_on(device: torch.device) -> int:
+    """The current stream, as an integer. Calls launch on the current device: buffers of another one are refused, not touched."""
     if device.type != "cuda":
         raise ValueError(f"the buffers are on {device}, not on a CUDA device")
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"the buffers are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    index = _current_index()
+    if device.index != index:
+        raise ValueError(f"the buffers are on {device}, the current device is cuda:{index}")
+    return torch.cuda.current_stream().cuda_stream if _raw_stream_of_device is None else _raw_stream_of_device(index)
 
 
 class Rotary:
@@ -313,30 +321,36 @@ class KvCache:
                positions: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
         """Writes the batch's new tokens, k and v [tokens, kv_heads * head_dim], to its pages, keys turned by `rotary`; returns the queries
         q [tokens, heads * head_dim] turned the same way (bf16 where q_out does not say otherwise), None without q."""
-        T, width = batch.tokens, self.kv_heads * self.head_dim
-        _here(self.device)
-        if batch.device != self.device:
-            raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
-        ld_k, ld_v = _rows(k, T, width, "k", self.device), _rows(v, T, width, "v", self.device)
+        T, width, device = batch.tokens, self.kv_heads * self.head_dim, self.device
+        stream = _stream_on(device)
+        if batch.device != device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {device}")
+        ld_k, ld_v = _rows(k, T, width, "k", device), _rows(v, T, width, "v", device)
         dt = _dtype(k, "k")
         if v.dtype != k.dtype:
             raise TypeError("k and v of one type")
-        heads = ld_q = ld_o = 0
+        heads = ld_q = ld_o = turned = interleaved = 0
         q_dt = o_dt = abi.BF16
+        q_at = o_at = positions_at = frequencies_at = None
         if q is not None:
-            heads = q.shape[1] // self.head_dim
-            ld_q, q_dt = _rows(q, T, heads * self.head_dim, "q", self.device), _dtype(q, "q")
+            heads = q.shape[-1] // self.head_dim
+            q_width = heads * self.head_dim
+            ld_q, q_dt, q_at = _rows(q, T, q_width, "q", device), _dtype(q, "q"), q.data_ptr()
             if q_out is None:
-                q_out = torch.empty((T, heads * self.head_dim), dtype=torch.bfloat16, device=q.device)
-            ld_o, o_dt = _rows(q_out, T, heads * self.head_dim, "q_out", self.device), _dtype(q_out, "q_out")
-        if positions is not None and (positions.dtype != torch.int32 or tuple(positions.shape) != (T,) or not positions.is_contiguous() or positions.device != self.device):
-            raise ValueError(f"positions: contiguous int32 [{T}] on {self.device}")
-        if rotary is not None and rotary.frequencies.device != self.device:
-            raise ValueError(f"the frequencies are on {rotary.frequencies.device}, the cache on {self.device}")
-        st = self.lib.lx_b200_kv_append(self.address, batch.address, k.data_ptr(), ld_k, v.data_ptr(), ld_v, dt, q.data_ptr() if q is not None else None, q_dt,
-                                        ld_q, heads, q_out.data_ptr() if q is not None else None, o_dt, ld_o,
-                                        positions.data_ptr() if positions is not None else None, rotary.frequencies.data_ptr() if rotary is not None else None,
-                                        rotary.dim if rotary is not None else 0, int(rotary is not None and rotary.interleaved), _raw_stream())
+                q_out, ld_o = torch.empty((T, q_width), dtype=torch.bfloat16, device=device), q_width
+            else:
+                ld_o, o_dt = _rows(q_out, T, q_width, "q_out", device), _dtype(q_out, "q_out")
+            o_at = q_out.data_ptr()
+        if positions is not None:
+            if positions.dtype is not torch.int32 or positions.shape != (T,) or not positions.is_contiguous() or positions.device != device:
+                raise ValueError(f"positions: contiguous int32 [{T}] on {device}")
+            positions_at = positions.data_ptr()
+        if rotary is not None:
+            if rotary.frequencies.device != device:
+                raise ValueError(f"the frequencies are on {rotary.frequencies.device}, the cache on {device}")
+            frequencies_at, turned, interleaved = rotary.frequencies.data_ptr(), rotary.dim, int(rotary.interleaved)
+        st = self.lib.lx_b200_kv_append(self.address, batch.address, k.data_ptr(), ld_k, v.data_ptr(), ld_v, dt, q_at, q_dt, ld_q, heads, o_at, o_dt, ld_o,
+                                        positions_at, frequencies_at, turned, interleaved, stream)
         if st:
             raise RuntimeError(f"lx_b200_kv_append failed: {st}")
         return q_out if q is not None else None
@@ -356,15 +370,17 @@ class Attention:
     def __call__(self, batch: KvBatch, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """q: f32 or bf16 [tokens, heads * head_dim]; out: bf16, the same shape (rows past the last sequence are left as they are)."""
         cache, T, width = self.cache, batch.tokens, self.heads * self.cache.head_dim
-        _here(cache.device)
-        if batch.device != cache.device:
-            raise ValueError(f"the batch is on {batch.device}, the cache on {cache.device}")
-        ld_q, dt = _rows(q, T, width, "q", cache.device), _dtype(q, "q")
+        device, ld_o = cache.device, width
+        stream = _stream_on(device)
+        if batch.device != device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {device}")
+        ld_q, dt = _rows(q, T, width, "q", device), _dtype(q, "q")
         if out is None:
-            out = torch.empty((T, width), dtype=torch.bfloat16, device=q.device)
-        elif out.dtype != torch.bfloat16:
+            out = torch.empty((T, width), dtype=torch.bfloat16, device=device)
+        elif out.dtype is not torch.bfloat16:
             raise TypeError("out: bfloat16")
-        ld_o = _rows(out, T, width, "out", cache.device)
+        else:
+            ld_o = _rows(out, T, width, "out", device)
         need = self._need.get(batch.sizes)
         if need is None:
             need = cache.lib.lx_b200_attention_workspace_bytes(cache.address, batch.address, self.heads)
@@ -372,9 +388,9 @@ class Attention:
                 raise RuntimeError("lx_b200_attention refuses this cache")
             if len(self._need) < 4096:
                 self._need[batch.sizes] = need
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
         st = cache.lib.lx_b200_attention(cache.address, batch.address, q.data_ptr(), dt, ld_q, self.heads, self.scale, self.window, out.data_ptr(), ld_o,
-                                         ws.data_ptr(), _raw_stream())
+                                         ws.data_ptr(), stream)
         if st:
             raise RuntimeError(f"lx_b200_attention failed: {st}")
         return out
@@ -395,41 +411,45 @@ class NormResidual:
                 self._weight_dt = _dtype(w, what)
         if pre is not None and post is not None and (pre.dtype != post.dtype or pre.device != post.device):
             raise ValueError("pre and post of one type on one device")
+        self._device = next((w.device for w in (pre, post) if w is not None), None)
+        self._pre_at, self._post_at = (None if w is None else w.data_ptr() for w in (pre, post))
 
     def __call__(self, y: torch.Tensor | None, h: torch.Tensor, gate: torch.Tensor | None = None, h_out: torch.Tensor | None = None,
                  x: torch.Tensor | None = None):
         """y: the block's output (None: nothing is added), h: the residual stream, both f32 or bf16 [T, width]; gate: [width] or [T, width].
         Returns the new residual stream, in h's type (h_out may be h), and the next block's input (bf16 where x does not say
         otherwise; None without a pre norm)."""
-        T, C = h.shape[0], self.width
-        _here(h.device)
-        ld_h, h_dt = _rows(h, T, C, "h"), _dtype(h, "h")
-        ld_y, y_dt = (0, abi.BF16) if y is None else (_rows(y, T, C, "y", h.device), _dtype(y, "y"))
-        ld_g, g_dt = 0, abi.BF16
+        T, C, device = h.shape[0], self.width, h.device
+        stream = _stream_on(device)
+        if self._device is not None and self._device != device:
+            raise ValueError(f"the weights are on {self._device}, the rows on {device}")
+        ld_h, h_dt = _rows(h, T, C, "h", device), _dtype(h, "h")
+        ld_y = ld_g = ld_x = 0
+        y_dt = g_dt = x_dt = abi.BF16
+        y_at = g_at = x_at = None
+        if y is not None:
+            ld_y, y_dt, y_at = _rows(y, T, C, "y", device), _dtype(y, "y"), y.data_ptr()
         if gate is not None:
-            g_dt = _dtype(gate, "gate")
+            g_dt, g_at = _dtype(gate, "gate"), gate.data_ptr()
             if gate.dim() == 2:
-                ld_g = _rows(gate, T, C, "gate", h.device)
-            elif tuple(gate.shape) != (C,) or (C > 1 and gate.stride(0) != 1) or gate.device != h.device:
-                raise ValueError(f"gate: [{C}] or [{T}, {C}] on {h.device}")
-        for w in (self.pre, self.post):
-            if w is not None and w.device != h.device:
-                raise ValueError(f"the weights are on {w.device}, the rows on {h.device}")
+                ld_g = _rows(gate, T, C, "gate", device)
+            elif gate.shape != (C,) or (gate.stride(0) != 1 and C > 1) or gate.device != device:
+                raise ValueError(f"gate: [{C}] or [{T}, {C}] on {device}")
         if h_out is None:
-            h_out = torch.empty((T, C), dtype=h.dtype, device=h.device)
-        elif h_out.dtype != h.dtype:
+            h_out, ld_ho = torch.empty((T, C), dtype=h.dtype, device=device), C
+        elif h_out.dtype is not h.dtype:
             raise TypeError("h_out of h's type")
-        ld_ho, ld_x, x_dt = _rows(h_out, T, C, "h_out", h.device), 0, abi.BF16
-        if self.pre is not None:
-            if x is None:
-                x = torch.empty((T, C), dtype=torch.bfloat16, device=h.device)
-            ld_x, x_dt = _rows(x, T, C, "x", h.device), _dtype(x, "x")
         else:
+            ld_ho = _rows(h_out, T, C, "h_out", device)
+        if self.pre is None:
             x = None
-        st = self.lib.lx_b200_norm_residual(y.data_ptr() if y is not None else None, y_dt, ld_y, h.data_ptr(), h_dt, ld_h, gate.data_ptr() if gate is not None else None,
-                                            g_dt, ld_g, self.gate_sigmoid, self.post.data_ptr() if self.post is not None else None,
-                                            self.pre.data_ptr() if self.pre is not None else None, self._weight_dt, self.residual_scale, self.block_scale, self.eps,
-                                            h_out.data_ptr(), ld_ho, x.data_ptr() if x is not None else None, x_dt, ld_x, T, C, _raw_stream())
+        elif x is None:
+            x, ld_x = torch.empty((T, C), dtype=torch.bfloat16, device=device), C
+            x_at = x.data_ptr()
+        else:
+            ld_x, x_dt, x_at = _rows(x, T, C, "x", device), _dtype(x, "x"), x.data_ptr()
+        st = self.lib.lx_b200_norm_residual(y_at, y_dt, ld_y, h.data_ptr(), h_dt, ld_h, g_at, g_dt, ld_g, self.gate_sigmoid, self._post_at, self._pre_at,
+                                            self._weight_dt, self.residual_scale, self.block_scale, self.eps, h_out.data_ptr(), ld_ho, x_at, x_dt, ld_x, T, C, stream)
         if st:
             raise RuntimeError(f"lx_b200_norm_residual failed: {st}")
         return h_out, x

@@ -129,11 +129,14 @@ def test_the_host_refuses_buffers_that_do_not_fit(lib):
 
 
 def test_row_strides():
-    x = torch.zeros((4, 24))
-    assert host._rows(x[:, :8], 4, 8, "x") == 24 and host._rows(x[:1, :8], 1, 8, "x") == 24 and host._rows(x[:, :24], 4, 24, "x") == 24
-    for bad in (x[:, ::2], x[:2], x[:, :7], x[0]):
+    x, cpu = torch.zeros((4, 24)), torch.device("cpu")
+    assert host._rows(x[:, :8], 4, 8, "x", cpu) == 24 and host._rows(x[:1, :8], 1, 8, "x", cpu) == 24 and host._rows(x[:, :24], 4, 24, "x", cpu) == 24
+    assert host._rows(x[:1, :1], 1, 1, "x", cpu) == 24 and host._rows(x[:, ::24], 4, 1, "x", cpu) == 24
+    for bad in (x[:, ::2], x[:2], x[:, :7], x[:, None]):
         with pytest.raises(ValueError):
-            host._rows(bad, 4, 12, "x")
+            host._rows(bad, 4, 12, "x", cpu)
+    with pytest.raises(ValueError):
+        host._rows(x, 4, 24, "x", torch.device("cuda", 0))
 
 
 # ---- the plain implementations -------------------------------------------------------------------------------------------------
