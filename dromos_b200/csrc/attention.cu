@@ -76,7 +76,7 @@ __device__ Place find_tile(const AttentionArgs& A, int64_t piece, int pieces, in
       if (pass == 0) total += all;
       if (pass == 1 || whole) {
         if (whole) {
-          per = max(static_cast<int64_t>(A.min_tiles), (total + pieces - 1) / pieces);
+          per = max(static_cast<int64_t>(A.min_tiles), divide(total + pieces - 1, pieces));
           at = piece * per;
         }
         if (base + incl > at && base + incl - mine <= at) shared->seq = s0 + tid, shared->base = base + incl - mine;
@@ -86,7 +86,7 @@ __device__ Place find_tile(const AttentionArgs& A, int64_t piece, int pieces, in
       }
     }
     if (pass == 0) {
-      per = max(static_cast<int64_t>(A.min_tiles), (total + pieces - 1) / pieces);
+      per = max(static_cast<int64_t>(A.min_tiles), divide(total + pieces - 1, pieces));
       at = piece * per;
     }
   }
@@ -166,48 +166,18 @@ __global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3
       continue;
     }
     // this CTA's part of one unit
-    const int unit = static_cast<int>((at - base) / W.tiles);
+    const int unit = static_cast<int>(divide(at - base, W.tiles));
     const int64_t unit_at = base + static_cast<int64_t>(unit) * W.tiles;
     const int part0 = static_cast<int>(at - unit_at), part1 = static_cast<int>(min(static_cast<int64_t>(W.tiles), end - unit_at));
     const int head = unit % C.kv_heads, row_block = unit / C.kv_heads * ROWS, rows = min(ROWS, W.q.n * A.group - row_block);
     const int first = W.q.length - W.q.n;
-    // queries: each row times the power of two that brings it into f16's range
-    for (int r = warp; r < ROWS; r += kWarps) {
-      const int token = (row_block + r) / A.group, qh = head * A.group + (row_block + r) % A.group;
-      float v[(D + 127) / 128][4], most = 0.0f;
-#pragma unroll
-      for (int i = 0; i < (D + 127) / 128; ++i) {
-        const int d = 4 * lane + 128 * i;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[i][j] = 0.0f;
-        if (r < rows && d < D) {
-          const int64_t src = (W.q.row0 + token) * A.ld_q + static_cast<int64_t>(qh) * D + d;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[i][j] = load_f32(A.q, A.q_dtype, src + j);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[i][j]));
-      }
-      const float up = f16_scale(warp_max(most));
-#pragma unroll
-      for (int i = 0; i < (D + 127) / 128; ++i) {
-        const int d = 4 * lane + 128 * i;
-        if (d >= D) continue;
-        const __half2 a = __floats2half2_rn(v[i][0] * up, v[i][1] * up), b = __floats2half2_rn(v[i][2] * up, v[i][3] * up);
-        qfrag[(d % (D / 4) / 4 * NT + r / 8) * 32 + r % 8 * 4 + d / (D / 4)] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-      }
-      if (lane == 0) rowf[r] = A.scale_log2 / up;
-    }
-    __syncthreads();
-    // what lane (g, t) knows of its rows 8 nt + 2 t and + 1: the factor of their scores, the first slot past what they see
-    float f[NT][2];
+    // what lane (g, t) knows of its rows 8 nt + 2 t and + 1: the first slot past what they see
     int past[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * nt + 2 * t4 + e;
-        f[nt][e] = rowf[r];
         past[nt][e] = r < rows ? first + (row_block + r) / A.group + 1 : 0;
       }
     const int past_low = first + row_block / A.group + 1, past_high = first + (row_block + rows - 1) / A.group + 1;  // of the first and the last row
@@ -250,6 +220,41 @@ __global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3
       load_k(src), load_v(src);
       sc = step_scale(A, page, head);
     }
+    // queries, while the first keys and values are on their way: each row times the power of two that brings it into f16's range
+    {
+      constexpr int PIECES = (D + 127) / 128, PER_WARP = ROWS / kWarps;
+      float4 x[PER_WARP * PIECES];
+      int64_t from[PER_WARP * PIECES];
+#pragma unroll
+      for (int i = 0; i < PER_WARP; ++i) {  // rows past the end: the last one, so that no load waits for a condition
+        const int r = row_block + min(warp + kWarps * i, rows - 1);
+        const int64_t src = (W.q.row0 + r / A.group) * A.ld_q + (static_cast<int64_t>(head) * A.group + r % A.group) * D;
+#pragma unroll
+        for (int b = 0; b < PIECES; ++b) from[i * PIECES + b] = src + (4 * lane + 128 * b) % D;
+      }
+      load_rows4(A.q, A.q_dtype, from, A.q_vec, x);
+#pragma unroll
+      for (int i = 0; i < PER_WARP; ++i) {
+        const int r = warp + kWarps * i;
+        float most = 0.0f;
+#pragma unroll
+        for (int b = 0; b < PIECES; ++b) most = fmaxf(fmaxf(fmaxf(most, fabsf(x[i * PIECES + b].x)), fabsf(x[i * PIECES + b].y)), fmaxf(fabsf(x[i * PIECES + b].z), fabsf(x[i * PIECES + b].w)));
+        const float up = f16_scale(warp_max(most));
+#pragma unroll
+        for (int b = 0; b < PIECES; ++b) {
+          const int d = 4 * lane + 128 * b;
+          if (d >= D) continue;
+          const float4 q = r < rows ? x[i * PIECES + b] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          const __half2 lo = __floats2half2_rn(q.x * up, q.y * up), hi = __floats2half2_rn(q.z * up, q.w * up);
+          qfrag[(d % (D / 4) / 4 * NT + r / 8) * 32 + r % 8 * 4 + d / (D / 4)] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        }
+        if (lane == 0) rowf[r] = A.scale_log2 / up;
+      }
+    }
+    __syncthreads();
+    float f[NT][2];  // the factors of the rows' scores
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) f[nt][0] = rowf[8 * nt + 2 * t4], f[nt][1] = rowf[8 * nt + 2 * t4 + 1];
     for (; step < step_end; step += kWarps) {
       const int slot = step * 16;
       // scores
@@ -408,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3
 template <int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttentionArgs A) {
   constexpr int ROWS = 8 * NT, AT_ONCE = 32, ITEMS = (ROWS * (D / 4) + kJoinThreads - 1) / kJoinThreads;
-  __shared__ float ms[AT_ONCE][ROWS], ls[AT_ONCE][ROWS], shrink[ROWS], sums[ROWS], tops[ROWS];
+  __shared__ float ms[AT_ONCE][ROWS + 1], ls[AT_ONCE][ROWS + 1], shrink[ROWS], sums[ROWS], tops[ROWS];
   pdl_wait();
   const JoinInfo u = A.join[blockIdx.x];
   if (u.rows == 0) return;
@@ -427,18 +432,15 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
       if (i % ROWS < u.rows) ms[i / ROWS][i % ROWS] = src[0], ls[i / ROWS][i % ROWS] = src[ROWS];
     }
     __syncthreads();
-    if (tid < u.rows) {
-      float top = tops[tid], sum = sums[tid];
-      for (int p = 0; p < n; ++p) top = fmaxf(top, ms[p][tid]);
-      shrink[tid] = tops[tid] == -INFINITY ? 0.0f : exp2_fast(tops[tid] - top);
+    for (int r = tid >> 5; r < u.rows; r += kJoinThreads / 32) {  // a lane for each part
+      const int p = tid & 31;
+      const float m = p < n ? ms[p][r] : -INFINITY, l = p < n ? ls[p][r] : 0.0f, before = tops[r], top = fmaxf(before, warp_max(m));
       // a part whose scores were all not-a-number has no maximum, its sums say so
-      sum = tops[tid] == -INFINITY ? sum : sum * shrink[tid];
-      for (int p = 0; p < n; ++p) {
-        const float m = ms[p][tid], k = m == -INFINITY ? 0.0f : exp2_fast(m - top);
-        sum += m == -INFINITY ? ls[p][tid] : ls[p][tid] * k;
-        ms[p][tid] = k;
-      }
-      tops[tid] = top, sums[tid] = sum;
+      const float k = m == -INFINITY ? 0.0f : exp2_fast(m - top), gain = warp_sum(m == -INFINITY ? l : l * k);
+      const float k0 = before == -INFINITY ? 0.0f : exp2_fast(before - top);
+      if (p < n) ms[p][r] = k;
+      __syncwarp();
+      if (p == 0) shrink[r] = k0, tops[r] = top, sums[r] = (before == -INFINITY ? sums[r] : sums[r] * k0) + gain;
     }
     __syncthreads();
 #pragma unroll
@@ -447,11 +449,17 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
       if (r >= u.rows) continue;
       const float k0 = shrink[r];
       v[i] = make_float4(v[i].x * k0, v[i].y * k0, v[i].z * k0, v[i].w * k0);
-#pragma unroll 8
-      for (int p = 0; p < n; ++p) {
-        const float4 o = *reinterpret_cast<const float4*>(slot(p0 + p) + 2 * ROWS + r * D + d);
-        const float k = ms[p][r];
-        v[i].x = fmaf(o.x, k, v[i].x), v[i].y = fmaf(o.y, k, v[i].y), v[i].z = fmaf(o.z, k, v[i].z), v[i].w = fmaf(o.w, k, v[i].w);
+#pragma unroll 1
+      for (int q0 = 0; q0 < n; q0 += 16) {
+        float4 o[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) o[q] = *reinterpret_cast<const float4*>(slot(p0 + min(q0 + q, n - 1)) + 2 * ROWS + r * D + d);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          if (q0 + q >= n) break;
+          const float k = ms[q0 + q][r];
+          v[i].x = fmaf(o[q].x, k, v[i].x), v[i].y = fmaf(o[q].y, k, v[i].y), v[i].z = fmaf(o[q].z, k, v[i].z), v[i].w = fmaf(o[q].w, k, v[i].w);
+        }
       }
     }
   }
@@ -551,7 +559,7 @@ extern "C" int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv
   A.kv = view_of(*cache, *batch);
   A.q = q, A.out = static_cast<uint16_t*>(out), A.ld_q = ld_q, A.ld_out = ld_out, A.partial = static_cast<float*>(workspace);
   A.q_dtype = q_dtype, A.q_heads = q_heads, A.group = q_heads / cache->kv_heads, A.window = window;
-  A.out_vec = aligned(out, 8) && ld_out % 4 == 0;
+  A.out_vec = aligned(out, 8) && ld_out % 4 == 0, A.q_vec = aligned(q, q_dtype == LX_BF16 ? 8 : 16) && ld_q % 4 == 0;
   A.scale_log2 = scale * 1.4426950408889634f;
   A.min_tiles = 2;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

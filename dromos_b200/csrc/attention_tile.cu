@@ -170,7 +170,7 @@ __device__ __forceinline__ bool next_part(const TileArgs& T, Share& w, Part& p) 
     int cost = b.tiles + kBlockCost;
     while (w.at >= b.before + static_cast<int64_t>(cost) * heads) b = T.plan[++w.block], cost = b.tiles + kBlockCost;
     const int64_t in = w.at - b.before;
-    p.s = b.s, p.row_block = b.row_block, p.head = static_cast<int>(in / cost);
+    p.s = b.s, p.row_block = b.row_block, p.head = static_cast<int>(divide(in, cost));
     const int64_t u0 = b.before + static_cast<int64_t>(p.head) * cost;
     const int c0 = static_cast<int>(w.at - u0), c1 = static_cast<int>(min(static_cast<int64_t>(cost), w.end - u0));
     w.at = u0 + c1;
@@ -190,14 +190,30 @@ __device__ __forceinline__ bool next_part(const TileArgs& T, Share& w, Part& p) 
 }
 
 // ---- tensor memory and products -----------------------------------------------------------------------------------------------
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+// Reads of tensor memory with their wait in one statement: the registers fill behind the compiler's back, and a copy that it made of
+// them between the two would have what was there before.
+__device__ __forceinline__ void tmem_ld_2x32(uint32_t taddr, uint32_t (&r)[2][32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
-      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0][0]), "=r"(r[0][1]), "=r"(r[0][2]), "=r"(r[0][3]), "=r"(r[0][4]), "=r"(r[0][5]), "=r"(r[0][6]), "=r"(r[0][7]), "=r"(r[0][8]), "=r"(r[0][9]), "=r"(r[0][10]), "=r"(r[0][11]), "=r"(r[0][12]), "=r"(r[0][13]), "=r"(r[0][14]), "=r"(r[0][15]), "=r"(r[0][16]), "=r"(r[0][17]), "=r"(r[0][18]), "=r"(r[0][19]), "=r"(r[0][20]), "=r"(r[0][21]), "=r"(r[0][22]), "=r"(r[0][23]), "=r"(r[0][24]), "=r"(r[0][25]), "=r"(r[0][26]), "=r"(r[0][27]), "=r"(r[0][28]), "=r"(r[0][29]), "=r"(r[0][30]), "=r"(r[0][31]),
+        "=r"(r[1][0]), "=r"(r[1][1]), "=r"(r[1][2]), "=r"(r[1][3]), "=r"(r[1][4]), "=r"(r[1][5]), "=r"(r[1][6]), "=r"(r[1][7]), "=r"(r[1][8]), "=r"(r[1][9]), "=r"(r[1][10]), "=r"(r[1][11]), "=r"(r[1][12]), "=r"(r[1][13]), "=r"(r[1][14]), "=r"(r[1][15]), "=r"(r[1][16]), "=r"(r[1][17]), "=r"(r[1][18]), "=r"(r[1][19]), "=r"(r[1][20]), "=r"(r[1][21]), "=r"(r[1][22]), "=r"(r[1][23]), "=r"(r[1][24]), "=r"(r[1][25]), "=r"(r[1][26]), "=r"(r[1][27]), "=r"(r[1][28]), "=r"(r[1][29]), "=r"(r[1][30]), "=r"(r[1][31])
+      : "r"(taddr), "r"(taddr + 32)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_4x16(uint32_t taddr, uint32_t step, uint32_t (&r)[4][16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%64];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%65];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47}, [%66];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%67];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0][0]), "=r"(r[0][1]), "=r"(r[0][2]), "=r"(r[0][3]), "=r"(r[0][4]), "=r"(r[0][5]), "=r"(r[0][6]), "=r"(r[0][7]), "=r"(r[0][8]), "=r"(r[0][9]), "=r"(r[0][10]), "=r"(r[0][11]), "=r"(r[0][12]), "=r"(r[0][13]), "=r"(r[0][14]), "=r"(r[0][15]),
+        "=r"(r[1][0]), "=r"(r[1][1]), "=r"(r[1][2]), "=r"(r[1][3]), "=r"(r[1][4]), "=r"(r[1][5]), "=r"(r[1][6]), "=r"(r[1][7]), "=r"(r[1][8]), "=r"(r[1][9]), "=r"(r[1][10]), "=r"(r[1][11]), "=r"(r[1][12]), "=r"(r[1][13]), "=r"(r[1][14]), "=r"(r[1][15]),
+        "=r"(r[2][0]), "=r"(r[2][1]), "=r"(r[2][2]), "=r"(r[2][3]), "=r"(r[2][4]), "=r"(r[2][5]), "=r"(r[2][6]), "=r"(r[2][7]), "=r"(r[2][8]), "=r"(r[2][9]), "=r"(r[2][10]), "=r"(r[2][11]), "=r"(r[2][12]), "=r"(r[2][13]), "=r"(r[2][14]), "=r"(r[2][15]),
+        "=r"(r[3][0]), "=r"(r[3][1]), "=r"(r[3][2]), "=r"(r[3][3]), "=r"(r[3][4]), "=r"(r[3][5]), "=r"(r[3][6]), "=r"(r[3][7]), "=r"(r[3][8]), "=r"(r[3][9]), "=r"(r[3][10]), "=r"(r[3][11]), "=r"(r[3][12]), "=r"(r[3][13]), "=r"(r[3][14]), "=r"(r[3][15])
+      : "r"(taddr), "r"(taddr + step), "r"(taddr + 2 * step), "r"(taddr + 3 * step)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -344,8 +360,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 
 // EDGE: some row of the warps does not see all of a tile; this one sees its slots lo <= j < hi. The loops stay rolled and read the
-// scores from tensor memory 32 at a time, the next ones while these are worked on: 128 scores in registers and straight code for
-// them ran at the rate of the instruction cache (a tile's weights 2100 cycles).
+// scores from tensor memory 64 at a time: 128 scores in registers and straight code for them ran at the rate of the instruction
+// cache. (The next scores read while the last ones are worked on would hide more, but nothing may stand between a read and its wait.)
 template <bool EDGE>
 __device__ __forceinline__ void mask_scores(uint32_t (&u)[32], int at, int lo, int hi) {
   if constexpr (EDGE) {
@@ -358,15 +374,13 @@ __device__ __forceinline__ void mask_scores(uint32_t (&u)[32], int at, int lo, i
 template <bool EDGE, int KT>
 __device__ __forceinline__ float tile_top(uint32_t s_tmem, const float4* sc, float f, int lo, int hi) {
   float top = -INFINITY;
-  uint32_t u[2][32];
-  tmem_ld32(s_tmem, u[0]);
 #pragma unroll 1
   for (int c0 = 0; c0 < KT / 32; c0 += 2) {
+    uint32_t u[2][32];
+    tmem_ld_2x32(s_tmem + 32 * c0, u);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int c = c0 + e;
-      tmem_wait_ld();
-      if (c + 1 < KT / 32) tmem_ld32(s_tmem + 32 * (c + 1), u[1 - e]);
       mask_scores<EDGE>(u[e], 32 * c, lo, hi);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -389,16 +403,14 @@ __device__ __forceinline__ float tile_top(uint32_t s_tmem, const float4* sc, flo
 template <bool EDGE, int KT>
 __device__ __forceinline__ float tile_weights(uint32_t s_tmem, const float4* sc, float f, float from, int lo, int hi) {
   float l = 0.0f;
-  uint32_t u[2][32];
-  tmem_ld32(s_tmem, u[0]);
 #pragma unroll 1
   for (int c0 = 0; c0 < KT / 32; c0 += 2) {
+    uint32_t u[2][32];
+    tmem_ld_2x32(s_tmem + 32 * c0, u);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int c = c0 + e;
       uint32_t w[16];
-      tmem_wait_ld();
-      if (c + 1 < KT / 32) tmem_ld32(s_tmem + 32 * (c + 1), u[1 - e]);
       mask_scores<EDGE>(u[e], 32 * c, lo, hi);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -479,7 +491,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   Share share;
   {
     const PlanHeader h = *T.header;
-    share.per = max(static_cast<int64_t>(A.min_tiles), (h.total + gridDim.x - 1) / gridDim.x);
+    share.per = max(static_cast<int64_t>(A.min_tiles), divide(h.total + gridDim.x - 1, gridDim.x));
     share.at = blockIdx.x * share.per;
     share.end = min(h.total, share.at + share.per);
     share.block = find_block(T, h.blocks, h.total, share.at, &found);
@@ -664,14 +676,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           if (i > 0) {
             l *= shrink;
             // the scores of this tile came after the product of the tile before: nothing is at work on these sums
+#pragma unroll 1
+            for (int c = 0; c < D; c += 64) {
+              uint32_t v[4][16];
+              tmem_ld_4x16(o_tmem + c, 16, v);
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t v[16];
-              tmem_ld16(o_tmem + 16 * c, v);
-              tmem_wait_ld();
+              for (int e = 0; e < 4; ++e) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * shrink);
-              tmem_st16(o_tmem + 16 * c, v);
+                for (int j = 0; j < 16; ++j) v[e][j] = __float_as_uint(__uint_as_float(v[e][j]) * shrink);
+                tmem_st16(o_tmem + c + 16 * e, v[e]);
+              }
             }
           }
         }
@@ -705,9 +719,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
 #pragma unroll
         for (int k = 0; k < W / 16; ++k) {
           uint32_t u[4][16];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) tmem_ld16(o_tmem + 4 * W * h + W * j + 16 * k, u[j]);
-          tmem_wait_ld();
+          tmem_ld_4x16(o_tmem + 4 * W * h + 16 * k, W, u);
           if (valid) {
 #pragma unroll
             for (int q = 0; q < 16; q += 4) {
@@ -777,6 +789,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
               for (int b = 0; b < PIECES / 4; ++b) x[a][b] = make_uint4(x[a][b].x & k, x[a][b].y & k, x[a][b].z & k, x[a][b].w & k);
             }
           }
+          proxy_fence();  // the codes have arrived in registers before a copy may write over them (without it some had not)
           warp_arrive(raw_empty + 8 * (n % RS));
           if (!warp_wait(k_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
             ok = false;
@@ -825,6 +838,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 for (int h = 0; h < HALVES; ++h) x[a][h][j] &= k;
               }
           }
+          proxy_fence();
           warp_arrive(raw_empty + 8 * (RS + n % RS));
           if (!warp_wait(v_empty + 8 * (n % NS), (n / NS & 1) ^ 1, V.status)) {
             ok = false;

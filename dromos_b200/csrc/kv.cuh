@@ -52,6 +52,29 @@ __device__ __forceinline__ float4 load_row4(const void* p, int dtype, int64_t i,
   return make_float4(load_f32(p, dtype, i), load_f32(p, dtype, i + 1), load_f32(p, dtype, i + 2), load_f32(p, dtype, i + 3));
 }
 
+// The same of N rows at once: every load is issued before one is waited for, which a choice of the type within each does not do.
+template <int N>
+__device__ __forceinline__ void load_rows4(const void* p, int dtype, const int64_t (&at)[N], bool vec, float4 (&x)[N]) {
+  if (vec && dtype == LX_BF16) {
+    uint2 w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      x[i] = make_float4(__uint_as_float(w[i].x << 16), __uint_as_float(w[i].x & 0xffff0000u), __uint_as_float(w[i].y << 16), __uint_as_float(w[i].y & 0xffff0000u));
+  } else if (vec) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = load_row4(p, dtype, at[i], false);
+  }
+}
+// a / b of counts: 64-bit division is a hundred instructions, and hardly ever needed.
+__device__ __forceinline__ int64_t divide(int64_t a, int b) {
+  return a >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
+
 // ---- host -----------------------------------------------------------------------------------------------------------
 inline int check_cache(const lx_b200_kv_cache* c) {
   if (!c || c->kv_heads < 1 || c->pages < 1 || !c->k || !c->v || !c->k_scale || !c->v_scale) return kInvalid;

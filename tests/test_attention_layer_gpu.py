@@ -255,6 +255,18 @@ def test_attention_over_long_caches(lx, new, total, window):
     check_attention(lx, S, 1, 4, 128, "fp8", window=window, spread=4.0)
 
 
+@pytest.mark.parametrize("new,total,D,K,G", [([257], [900], 64, 2, 7), ([300], [1500], 128, 1, 33), ([100, 130], [700, 800], 256, 2, 3), ([1, 1, 1], [900, 40, 3000], 128, 2, 4)])
+def test_attention_gives_the_same_bits_in_many_calls(lx, new, total, D, K, G):
+    """A copy that writes over what is still read, or a role that runs ahead of another, shows in one call of some hundred."""
+    S = R.Sequences(new, total, 32, seed=1)
+    cache, _ = make_cache(lx, S, K, D, "int8", 3)
+    q, attend, batch = normal((S.rows, K * G * D), 5, dtype=torch.bfloat16).cuda(), host.Attention(cache, K * G), put(S)
+    first = attend(batch, q)
+    outs = [attend(batch, q) for _ in range(600)]
+    util.check_status(lx)
+    assert all(torch.equal(o, first) for o in outs)
+
+
 @pytest.mark.parametrize("max_new", [0, 1, 8, 10**6])
 def test_attention_of_more_or_fewer_tokens_than_the_hint(lx, max_new):
     S = R.Sequences([150, 1, 9], [400, 100, 9], 16, seed=4)
