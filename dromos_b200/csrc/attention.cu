@@ -14,7 +14,7 @@ namespace b200 {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 512;
 constexpr int kTile = 16 * kWarps;  // slots of a tile: 16 for each warp
 
 // Work of a sequence: units (blocks of ROWS query rows x key heads) of equally many tiles.
@@ -124,6 +124,12 @@ __device__ __forceinline__ StepScale step_scale(const AttentionArgs& A, int page
   return {A.kv.k_scale[at], v, 0.0f};
 }
 
+// CTAs of an SM: what the accumulators' registers leave room for. (256 values per head: three CTAs spill, 24 sequences 45 us for 43.)
+template <int D, int NT>
+constexpr int stream_ctas() {
+  return D == 256 ? 2 : NT * D <= 128 ? 4 : NT * D <= 256 ? 3 : 2;
+}
+
 // NT groups of 8 query rows against the keys of one head. D: values of a head.
 //
 // A warp takes 16 slots at a time. Both products have the keys as the 16-row operand and the query rows as the 8 columns, so that a
@@ -132,7 +138,7 @@ __device__ __forceinline__ StepScale step_scale(const AttentionArgs& A, int page
 // product, the queries are laid out to match), and of values the dims g D/8 .. of slots 2t, 2t + 1, 2t + 8, 2t + 9, whose bytes are
 // interleaved before they are widened. P^T turns from accumulator to operand by one movmatrix per 8 x 8.
 template <bool kInt8, int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3 : 2) attention_stream_kernel(const __grid_constant__ AttentionArgs A) {
+__global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stream_kernel(const __grid_constant__ AttentionArgs A) {
   constexpr int ROWS = 8 * NT, KW = D / 16, VW = D / 32, MT = D / 16;
   constexpr int OS = D + 4;  // row stride of the accumulators in shared memory
   extern __shared__ __align__(16) uint8_t smem[];
@@ -149,11 +155,8 @@ __global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   int64_t per, at;
   const Place start = find_tile<ROWS>(A, blockIdx.x, gridDim.x, per, at, &place, sums);
-  JoinInfo join{};
-  if (start.seq < 0) {
-    if (tid == 0) A.join[blockIdx.x] = join;
-    return;
-  }
+  if (tid == 0) A.join[blockIdx.x].rows = 0;  // so far
+  if (start.seq < 0) return;
   const int64_t end = min(start.total, at + per);
   int s = start.seq;
   int64_t base = start.base;
@@ -214,13 +217,7 @@ __global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3
       for (int i = 0; i < 4; ++i) load_codes(C.v + src + (2 * t4 + (i & 1) + 8 * (i >> 1)) * D + g * (D / 8), vw[i]);
     };
     int page = page_at(step), page_next = page_at(step + kWarps);
-    StepScale sc{};
-    if (step < step_end) {
-      const int64_t src = slot_base(page, step);
-      load_k(src), load_v(src);
-      sc = step_scale(A, page, head);
-    }
-    // queries, while the first keys and values are on their way: each row times the power of two that brings it into f16's range
+    // queries, while the table is read: each row times the power of two that brings it into f16's range
     {
       constexpr int PIECES = (D + 127) / 128, PER_WARP = ROWS / kWarps;
       float4 x[PER_WARP * PIECES];
@@ -250,6 +247,12 @@ __global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3
         }
         if (lane == 0) rowf[r] = A.scale_log2 / up;
       }
+    }
+    StepScale sc{};
+    if (step < step_end) {
+      const int64_t src = slot_base(page, step);
+      load_k(src), load_v(src);
+      sc = step_scale(A, page, head);
     }
     __syncthreads();
     float f[NT][2];  // the factors of the rows' scores
@@ -402,22 +405,23 @@ __global__ void __launch_bounds__(kThreads, NT* D <= 128 ? 4 : NT * D <= 256 ? 3
     }
     __syncthreads();  // before the next unit's queries and sums
     at = unit_at + part1;
-    if (part0 == 0 && !complete) join = {W.q.row0, row_block, rows, head, static_cast<int>((unit_at + W.tiles - 1) / per), {}};
+    if (part0 == 0 && !complete && tid == 0) A.join[blockIdx.x] = {W.q.row0, row_block, rows, head, static_cast<int>((unit_at + W.tiles - 1) / per), {}};
   }
-  if (tid == 0) A.join[blockIdx.x] = join;
 }
 
 // Joins the units that several CTAs of the stream kernel shared: CTA i the one that began in share i and went on into the next. The
-// parts' maxima and sums are looked at 32 parts at once, then their accumulators are read without one waiting for the other (a loop
-// that carried the maximum from part to part took decode of one sequence of 4099 tokens from 17 us to what the parts cost).
+// parts' maxima and sums are looked at 32 parts at once, a lane for each; their accumulators are read by as many groups of threads as
+// there are threads for (a part takes a thread 300 cycles, whatever is in flight beside it).
 template <int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttentionArgs A) {
-  constexpr int ROWS = 8 * NT, AT_ONCE = 32, ITEMS = (ROWS * (D / 4) + kJoinThreads - 1) / kJoinThreads;
+  constexpr int ROWS = 8 * NT, AT_ONCE = 32, CELLS = ROWS * (D / 4);  // four values each
+  constexpr int GROUPS = CELLS >= kJoinThreads ? 1 : kJoinThreads / CELLS, ITEMS = CELLS > kJoinThreads ? CELLS / kJoinThreads : 1;
   __shared__ float ms[AT_ONCE][ROWS + 1], ls[AT_ONCE][ROWS + 1], shrink[ROWS], sums[ROWS], tops[ROWS];
+  __shared__ float4 gathered[GROUPS > 1 ? GROUPS - 1 : 1][GROUPS > 1 ? CELLS : 1];
   pdl_wait();
   const JoinInfo u = A.join[blockIdx.x];
   if (u.rows == 0) return;
-  const int tid = threadIdx.x, first = blockIdx.x;
+  const int tid = threadIdx.x, first = blockIdx.x, group = GROUPS > 1 ? tid / CELLS : 0, cell0 = GROUPS > 1 ? tid % CELLS : tid;
   const int64_t slot_floats = ROWS * (D + 2);
   auto slot = [&](int p) { return A.partial + (2 * static_cast<int64_t>(p) + (p == first)) * slot_floats; };
   if (tid < ROWS) sums[tid] = 0.0f, tops[tid] = -INFINITY;
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
       if (i % ROWS < u.rows) ms[i / ROWS][i % ROWS] = src[0], ls[i / ROWS][i % ROWS] = src[ROWS];
     }
     __syncthreads();
-    for (int r = tid >> 5; r < u.rows; r += kJoinThreads / 32) {  // a lane for each part
+    for (int r = tid >> 5; r < u.rows; r += kJoinThreads / 32) {
       const int p = tid & 31;
       const float m = p < n ? ms[p][r] : -INFINITY, l = p < n ? ls[p][r] : 0.0f, before = tops[r], top = fmaxf(before, warp_max(m));
       // a part whose scores were all not-a-number has no maximum, its sums say so
@@ -445,37 +449,37 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int at = tid + i * kJoinThreads, r = at / (D / 4), d = at % (D / 4) * 4;
+      const int cell = cell0 + i * kJoinThreads, r = cell / (D / 4);
       if (r >= u.rows) continue;
       const float k0 = shrink[r];
       v[i] = make_float4(v[i].x * k0, v[i].y * k0, v[i].z * k0, v[i].w * k0);
-#pragma unroll 1
-      for (int q0 = 0; q0 < n; q0 += 16) {
-        float4 o[16];
-#pragma unroll
-        for (int q = 0; q < 16; ++q) o[q] = *reinterpret_cast<const float4*>(slot(p0 + min(q0 + q, n - 1)) + 2 * ROWS + r * D + d);
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          if (q0 + q >= n) break;
-          const float k = ms[q0 + q][r];
-          v[i].x = fmaf(o[q].x, k, v[i].x), v[i].y = fmaf(o[q].y, k, v[i].y), v[i].z = fmaf(o[q].z, k, v[i].z), v[i].w = fmaf(o[q].w, k, v[i].w);
-        }
+#pragma unroll 4
+      for (int p = group; p < n; p += GROUPS) {
+        const float4 o = *reinterpret_cast<const float4*>(slot(p0 + p) + 2 * ROWS + 4 * cell);
+        const float k = ms[p][r];
+        v[i].x = fmaf(o.x, k, v[i].x), v[i].y = fmaf(o.y, k, v[i].y), v[i].z = fmaf(o.z, k, v[i].z), v[i].w = fmaf(o.w, k, v[i].w);
       }
+    }
+  }
+  if constexpr (GROUPS > 1) {
+    if (group > 0) gathered[group - 1][cell0] = v[0];
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 0; g < GROUPS - 1; ++g) {
+      const float4 o = gathered[g][cell0];
+      v[0].x += o.x, v[0].y += o.y, v[0].z += o.z, v[0].w += o.w;
     }
   }
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const int at = tid + i * kJoinThreads, r = at / (D / 4), d = at % (D / 4) * 4;
+    const int cell = cell0 + i * kJoinThreads, r = cell / (D / 4);
     if (r >= u.rows) continue;
     const int token = (u.row_block + r) / A.group, qh = u.head * A.group + (u.row_block + r) % A.group;
-    store_out(A, (u.row0 + token) * A.ld_out + static_cast<int64_t>(qh) * D + d, v[i], sums[r] == 0.0f ? 0.0f : 0x1p-14f / sums[r]);
+    store_out(A, (u.row0 + token) * A.ld_out + static_cast<int64_t>(qh) * D + cell % (D / 4) * 4, v[i], sums[r] == 0.0f ? 0.0f : 0x1p-14f / sums[r]);
   }
 }
 
-template <int D, int NT>
-constexpr int stream_ctas() {
-  return NT * D <= 128 ? 4 : NT * D <= 256 ? 3 : 2;
-}
 template <int D, int NT>
 constexpr size_t stream_smem() {
   return D / 16 * NT * 32 * 8 + sizeof(float) * (kWarps * 8 * NT * (D + 4) + 2 * kWarps * 8 * NT + 8 * NT);
@@ -561,7 +565,7 @@ extern "C" int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv
   A.q_dtype = q_dtype, A.q_heads = q_heads, A.group = q_heads / cache->kv_heads, A.window = window;
   A.out_vec = aligned(out, 8) && ld_out % 4 == 0, A.q_vec = aligned(q, q_dtype == LX_BF16 ? 8 : 16) && ld_q % 4 == 0;
   A.scale_log2 = scale * 1.4426950408889634f;
-  A.min_tiles = 2;
+  A.min_tiles = 3;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool int8 = cache->type == LX_W_INT8;
   const AttentionPlan plan = attention_plan(*cache, *batch, A.group);

@@ -3,7 +3,10 @@
 //
 //   u = y rsqrt(mean y^2 + eps) post;   h' = residual_scale h + block_scale gate u;   x = h' rsqrt(mean h'^2 + eps) pre
 //
-// A row is one CTA's; a thread keeps its values in registers from the one read of y, h and gate to the writes of h' and x.
+// A row is one CTA's; a thread keeps its values in registers from the one read of y, h and gate to the writes of h' and x. Few rows are
+// a chain of latencies: all loads, the weights' among them, are issued at once (one row of 4096: 2.8 us). Many rows are bound by HBM,
+// and what counts is that one row of an SM loads while another one is summed: then the weights, which the caches hold, are read
+// where they are used, so that two CTAs of 512 threads fit the SM's registers. The same threads have the same values either way.
 #include <algorithm>
 
 #include "launch.cuh"
@@ -64,22 +67,22 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
 __device__ __forceinline__ float gate_of(float g, int sigmoid) { return sigmoid ? 1.0f / (1.0f + expf(-g)) : g; }
 
 // Rows of whole 16-byte-aligned pieces of eight values: thread t has the pieces t, t + blockDim.x, ... (PIECES of them at most).
-template <int PIECES>
-__global__ void __launch_bounds__(PIECES == 1 ? 1024 : 512) norm_kernel(const __grid_constant__ NormArgs A) {
+template <int PIECES, bool LATE>
+__global__ void __launch_bounds__(512, LATE ? (PIECES == 1 ? 3 : PIECES == 2 ? 2 : 1) : 1) norm_kernel(const __grid_constant__ NormArgs A) {
   __shared__ float part[2][32];
   pdl_wait();
   const int64_t row = blockIdx.x;
   const int pieces = A.C / 8;
-  Raw8 y[PIECES], h[PIECES], g[PIECES], wp[PIECES], wn[PIECES];
+  Raw8 y[PIECES], h[PIECES], g[LATE ? 1 : PIECES], wp[LATE ? 1 : PIECES], wn[LATE ? 1 : PIECES];
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int p = threadIdx.x + i * blockDim.x;
     if (p >= pieces) continue;
     if (A.y) y[i] = load_raw8(A.y, A.y_dtype, row * A.ld_y + 8 * p);
     h[i] = load_raw8(A.h, A.h_dtype, row * A.ld_h + 8 * p);
-    if (A.y && A.gate) g[i] = load_raw8(A.gate, A.gate_dtype, row * A.ld_gate + 8 * p);
-    if (A.y && A.post) wp[i] = load_raw8(A.post, A.weight_dtype, 8 * p);
-    if (A.pre) wn[i] = load_raw8(A.pre, A.weight_dtype, 8 * p);
+    if (!LATE && A.y && A.gate) g[i] = load_raw8(A.gate, A.gate_dtype, row * A.ld_gate + 8 * p);
+    if (!LATE && A.y && A.post) wp[i] = load_raw8(A.post, A.weight_dtype, 8 * p);
+    if (!LATE && A.pre) wn[i] = load_raw8(A.pre, A.weight_dtype, 8 * p);
   }
   float scale = A.block_scale;
   if (A.y && A.post) {
@@ -108,12 +111,12 @@ __global__ void __launch_bounds__(PIECES == 1 ? 1024 : 512) norm_kernel(const __
 #pragma unroll
       for (int j = 0; j < 8; ++j) u[j] *= scale;
       if (A.post) {
-        values_of(wp[i], A.weight_dtype, v);
+        values_of(LATE ? load_raw8(A.post, A.weight_dtype, 8 * p) : wp[LATE ? 0 : i], A.weight_dtype, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) u[j] *= v[j];
       }
       if (A.gate) {
-        values_of(g[i], A.gate_dtype, v);
+        values_of(LATE ? load_raw8(A.gate, A.gate_dtype, row * A.ld_gate + 8 * p) : g[LATE ? 0 : i], A.gate_dtype, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) u[j] *= gate_of(v[j], A.gate_sigmoid);
       }
@@ -131,7 +134,7 @@ __global__ void __launch_bounds__(PIECES == 1 ? 1024 : 512) norm_kernel(const __
     const int p = threadIdx.x + i * blockDim.x;
     if (p >= pieces) continue;
     float v[8];
-    values_of(wn[i], A.weight_dtype, v);
+    values_of(LATE ? load_raw8(A.pre, A.weight_dtype, 8 * p) : wn[LATE ? 0 : i], A.weight_dtype, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= next[i][j] * rms;
     store8(A.x, A.x_dtype, row * A.ld_x + 8 * p, v);
@@ -202,7 +205,10 @@ extern "C" int lx_b200_norm_residual(const void* y, lx_dtype y_dtype, int ld_y, 
   const bool pieces = C % 8 == 0 && whole(y, y_dtype, ld_y) && whole(h, h_dtype, ld_h) && whole(gate, gate_dtype, ld_gate) && whole(post, weight_dtype, 0) &&
                       whole(pre, weight_dtype, 0) && whole(h_out, h_dtype, ld_h_out) && whole(pre ? x : nullptr, x_dtype, ld_x);
   // how a row is dealt to threads goes by C alone, so a row's bits do not depend on the other rows
-  if (pieces && C <= 8 * 1024) return launch_kernel(norm_kernel<1>, dim3(T), dim3((C / 8 + 31) / 32 * 32), 0, s, A);
-  if (pieces && C <= 4 * 8 * 512) return launch_kernel(norm_kernel<4>, dim3(T), dim3(((C / 8 + 3) / 4 + 31) / 32 * 32), 0, s, A);
+  const bool late = T > 296;  // two rows for each SM: from here on rows wait for one another and not for their own loads
+  auto threads = [&](int per) { return dim3(((C / 8 + per - 1) / per + 31) / 32 * 32); };
+  if (pieces && C <= 8 * 512) return launch_kernel(late ? norm_kernel<1, true> : norm_kernel<1, false>, dim3(T), threads(1), 0, s, A);
+  if (pieces && C <= 16 * 512) return launch_kernel(late ? norm_kernel<2, true> : norm_kernel<2, false>, dim3(T), threads(2), 0, s, A);
+  if (pieces && C <= 32 * 512) return launch_kernel(late ? norm_kernel<4, true> : norm_kernel<4, false>, dim3(T), threads(4), 0, s, A);
   return launch_kernel(norm_any_kernel, dim3(T), dim3(std::min(1024, (C + 31) / 32 * 32)), 0, s, A);
 }

@@ -388,7 +388,7 @@ def test_attention_with_offsets_past_32_bits(lx):
 
 
 # ---- norms -------------------------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("T,C", [(1, 4096), (3, 8), (2, 1), (5, 1000), (33, 2048), (2, 8192), (3, 8200), (2, 16384), (2, 16392), (7, 4097)])
+@pytest.mark.parametrize("T,C", [(1, 4096), (3, 8), (2, 1), (5, 1000), (33, 2048), (2, 8192), (3, 8200), (2, 16384), (2, 16392), (7, 4097), (300, 4096), (310, 5000), (300, 16384)])
 @pytest.mark.parametrize("y,h,w,gate,sigmoid,post,x", [
     ("f32", "f32", "bf16", None, False, True, "bf16"), ("bf16", "bf16", "f32", "channel", False, True, "f32"), ("f32", "bf16", "bf16", "token", True, True, "bf16"),
     ("bf16", "f32", "f32", "token", False, False, "bf16"), (None, "f32", "bf16", None, False, False, "f32")])
