@@ -2,7 +2,7 @@
 //
 // A CTA has the new tokens of one page for one key head: it alone decides the page's scales for that head, so there are no atomics and
 // the codes do not depend on the order of anything. It reads its rows twice: once for their largest magnitudes, once (from the
-// caches) for their codes.
+// caches) for their codes. The queries of the heads that share the key head are other CTAs'.
 #include <algorithm>
 
 #include "kv.cuh"
@@ -81,17 +81,19 @@ __device__ __forceinline__ float scale_for(uint32_t magnitude, int int8) {
   return __uint_as_float(static_cast<uint32_t>(127 + min(max(want, kScaleMin), kScaleMax)) << 23);
 }
 
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendArgs A) {
+__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const __grid_constant__ AppendArgs A) {
   __shared__ float2 angles[kAnglePairs];
   __shared__ uint32_t most[2];
   pdl_wait();
   const KvView& C = A.kv;
-  const int s = blockIdx.x / A.splits, head = blockIdx.y, tid = threadIdx.x;
+  const int s = blockIdx.x / A.splits, tid = threadIdx.x;
+  const bool queries = blockIdx.y >= C.kv_heads;  // of the heads that share key head `head`, by CTAs of their own
+  const int head = queries ? blockIdx.y - C.kv_heads : blockIdx.y;
   bool bad;
   const Span q = span_of(C, s, bad);
   bad = bad || q.length < q.n;
   if (bad) {
-    if (tid == 0 && head == 0) report_batch(C);
+    if (tid == 0 && blockIdx.y == 0) report_batch(C);
     return;
   }
   if (q.n == 0) return;
@@ -100,10 +102,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
   for (int page = first / P + blockIdx.x % A.splits; page <= (q.length - 1) / P; page += A.splits) {
     const int lo = max(first, page * P), n = min(q.length, page * P + P) - lo, row0 = q.row0 + lo - first, kept = lo - page * P;
     const int at = page_of(C, s, page);
-    if (at < 0 && tid == 0 && head == 0) report_batch(C);
+    if (at < 0 && tid == 0 && blockIdx.y == 0) report_batch(C);
     if (tid < 2) most[tid] = 0;
     float now[2], inverse[2];
-    for (int pass = 0; pass < 2; ++pass) {
+    for (int pass = 0; pass < (queries ? 1 : 2); ++pass) {
       uint32_t large[2] = {0, 0};
       for (int c0 = 0; c0 < n; c0 += chunk) {
         const int m = min(chunk, n - c0);
@@ -121,7 +123,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
           }
         __syncthreads();
         const float2* cs = half ? angles : nullptr;
-        for (int i = tid; i < m * units; i += kAppendThreads) {
+        for (int i = tid; !queries && i < m * units; i += kAppendThreads) {
           const int t = i >> log_units;
           const Piece u = piece_of(A, i & (units - 1));
           const int64_t k_at = (row0 + c0 + t) * A.ld_k + head * D, v_at = (row0 + c0 + t) * A.ld_v + head * D;
@@ -148,16 +150,15 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
             *reinterpret_cast<uint32_t*>(C.v + dst + u.hi) = codes4(y + 4, A.int8);
           }
         }
-        if (pass == 0 && A.group > 0) {
-          // queries, four pieces of a thread on their way at once (one at a time left the memory idle: 12,000 tokens 101 us)
+        if (queries) {  // two pieces of a thread on their way at once
           const int all = m * A.group << log_units;
-          for (int i0 = tid; i0 < all; i0 += 4 * kAppendThreads) {
-            Piece u[4];
-            int token[4];
-            int64_t col[4], from[8];
-            float4 x[8];
+          for (int i0 = tid; i0 < all; i0 += 2 * kAppendThreads) {
+            Piece u[2];
+            int token[2];
+            int64_t col[2], from[4];
+            float4 x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 2; ++e) {
               const int i = min(i0 + e * kAppendThreads, all - 1), r = i >> log_units;
               token[e] = r / A.group;
               u[e] = piece_of(A, i & (units - 1));
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
             }
             load_rows4(A.q, A.q_dtype, from, A.q_vec, x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 2; ++e) {
               if (i0 + e * kAppendThreads >= all) break;
               float y[8];
               turn(A, x[2 * e], x[2 * e + 1], u[e], half ? cs + token[e] * half : nullptr, y);
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
           }
         }
       }
-      if (pass == 0) {
+      if (pass == 0 && !queries) {
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           large[w] = __reduce_max_sync(0xffffffffu, large[w]);
@@ -257,6 +258,6 @@ extern "C" int lx_b200_kv_append(const lx_b200_kv_cache* cache, const lx_b200_kv
   // CTAs per sequence and head: as many pages as max_new tokens reach at most (a sequence with more: its CTAs take several)
   const int P = cache->page_tokens, most = std::min(std::max(batch->max_new, 1), batch->tokens);
   A.splits = (most + P - 2) / P + 1;
-  return launch_kernel(kv_append_kernel, dim3(static_cast<unsigned>(batch->sequences) * A.splits, static_cast<unsigned>(H)), dim3(kAppendThreads), 0,
+  return launch_kernel(kv_append_kernel, dim3(static_cast<unsigned>(batch->sequences) * A.splits, static_cast<unsigned>(H) * (heads ? 2 : 1)), dim3(kAppendThreads), 0,
                        static_cast<cudaStream_t>(stream), A);
 }
