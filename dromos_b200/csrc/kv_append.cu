@@ -81,147 +81,170 @@ __device__ __forceinline__ float scale_for(uint32_t magnitude, int int8) {
   return __uint_as_float(static_cast<uint32_t>(127 + min(max(want, kScaleMin), kScaleMax)) << 23);
 }
 
+// Which pages a CTA has. With splits > 0 (batches whose sequences have about equally many new tokens) CTA x has the pages x % splits,
+// + splits, ... of sequence x / splits. Else it has place x of the batch: sequence s has starts[s] / P + 2 s .. starts[s + 1] / P +
+// 2 s + 1 of these, no fewer than the pages that its new tokens can touch, whatever slot they begin in. (A decode step of 64 sequences
+// takes 7.4 us the first way and 10.7 the second; a long prompt among 63 of them would leave 8,000 CTAs idle the first way.)
+__device__ __forceinline__ int places_before(const KvView& C, int s) { return min(max(C.starts[s], 0), C.tokens) / C.page_tokens + 2 * s; }
+
 __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const __grid_constant__ AppendArgs A) {
   __shared__ float2 angles[kAnglePairs];
   __shared__ uint32_t most[2];
+  __shared__ int next, matches;
   pdl_wait();
   const KvView& C = A.kv;
-  const int s = blockIdx.x / A.splits, tid = threadIdx.x;
+  const int tid = threadIdx.x, x = blockIdx.x;
   const bool queries = blockIdx.y >= C.kv_heads;  // of the heads that share key head `head`, by CTAs of their own
   const int head = queries ? blockIdx.y - C.kv_heads : blockIdx.y;
-  bool bad;
-  const Span q = span_of(C, s, bad);
-  bad = bad || q.length < q.n;
-  if (bad) {
-    if (tid == 0 && blockIdx.y == 0) report_batch(C);
-    return;
-  }
-  if (q.n == 0) return;
-  const int P = C.page_tokens, D = A.head_dim, log_units = __ffs(D) - 4, units = 1 << log_units, first = q.length - q.n, half = A.rotary / 2;
+  const int P = C.page_tokens, D = A.head_dim, log_units = __ffs(D) - 4, units = 1 << log_units, half = A.rotary / 2;
   const int chunk = half ? min(P, kAnglePairs / half) : P;
-  for (int page = first / P + blockIdx.x % A.splits; page <= (q.length - 1) / P; page += A.splits) {
-    const int lo = max(first, page * P), n = min(q.length, page * P + P) - lo, row0 = q.row0 + lo - first, kept = lo - page * P;
-    const int at = page_of(C, s, page);
-    if (at < 0 && tid == 0 && blockIdx.y == 0) report_batch(C);
-    if (tid < 2) most[tid] = 0;
-    float now[2], inverse[2];
-    for (int pass = 0; pass < (queries ? 1 : 2); ++pass) {
-      uint32_t large[2] = {0, 0};
-      for (int c0 = 0; c0 < n; c0 += chunk) {
-        const int m = min(chunk, n - c0);
-        __syncthreads();  // whoever still reads the angles, or `most`
-        if (half && (pass == 0 || n > chunk))
-          for (int i = tid; i < m * half; i += kAppendThreads) {
-            const int t = i / half;
-            const int position = A.positions ? A.positions[row0 + c0 + t] : lo + c0 + t;
-            // in turns, less the whole ones, before anything is rounded to f32: a position of a million costs no digits
-            double turns = static_cast<double>(position) * A.frequencies[i - t * half] * 0.15915494309189533577;
-            turns -= rint(turns);
-            float2 cs;
-            sincospif(2.0f * static_cast<float>(turns), &cs.y, &cs.x);
-            angles[i] = cs;
-          }
-        __syncthreads();
-        const float2* cs = half ? angles : nullptr;
-        for (int i = tid; !queries && i < m * units; i += kAppendThreads) {
-          const int t = i >> log_units;
-          const Piece u = piece_of(A, i & (units - 1));
-          const int64_t k_at = (row0 + c0 + t) * A.ld_k + head * D, v_at = (row0 + c0 + t) * A.ld_v + head * D;
-          float4 kx[2], vx[2];
-          const int64_t from_k[2] = {k_at + u.lo, k_at + u.hi}, from_v[2] = {v_at + u.lo, v_at + u.hi};
-          load_rows4(A.k, A.kv_dtype, from_k, A.k_vec, kx);
-          load_rows4(A.v, A.kv_dtype, from_v, A.v_vec, vx);
-          float x[8], y[8];
-          turn(A, kx[0], kx[1], u, half ? cs + t * half : nullptr, x);
-          turn(A, vx[0], vx[1], u, nullptr, y);
-          if (pass == 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              large[0] = max(large[0], __float_as_uint(x[j]) & 0x7fffffffu);  // as integers: not-a-number is the largest
-              large[1] = max(large[1], __float_as_uint(y[j]) & 0x7fffffffu);
+  // The sequence whose place this is; several only where the rows of sequences overlap, as they should not.
+  for (int s = -1, left = 1; left > 0; --left) {
+    if (A.splits > 0) {
+      s = x / A.splits;
+    } else {
+      __syncthreads();
+      if (tid == 0) next = INT_MAX, matches = 0;
+      __syncthreads();
+      for (int c = tid; c < C.sequences; c += kAppendThreads)
+        if (c > s && places_before(C, c) <= x && x < places_before(C, c + 1)) atomicMin(&next, c), atomicAdd(&matches, 1);
+      __syncthreads();
+      s = next, left = matches;
+      if (left == 0) break;
+    }
+    bool bad;
+    const Span q = span_of(C, s, bad);
+    if (bad || q.length < q.n || q.n == 0) continue;
+    const int first = q.length - q.n, place = A.splits > 0 ? x % A.splits : x - places_before(C, s), stride = A.splits > 0 ? A.splits : INT_MAX / 2;
+    for (int page = first / P + place; page <= (q.length - 1) / P; page += stride) {
+      const int lo = max(first, page * P), n = min(q.length, page * P + P) - lo, row0 = q.row0 + lo - first, kept = lo - page * P;
+      const int at = page_of(C, s, page);
+      if (at < 0 && tid == 0 && blockIdx.y == 0) report_batch(C);
+      if (tid < 2) most[tid] = 0;
+      float now[2], inverse[2];
+      for (int pass = 0; pass < (queries ? 1 : 2); ++pass) {
+        uint32_t large[2] = {0, 0};
+        for (int c0 = 0; c0 < n; c0 += chunk) {
+          const int m = min(chunk, n - c0);
+          __syncthreads();  // whoever still reads the angles, or `most`
+          if (half && (pass == 0 || n > chunk))
+            for (int i = tid; i < m * half; i += kAppendThreads) {
+              const int t = i / half;
+              const int position = A.positions ? A.positions[row0 + c0 + t] : lo + c0 + t;
+              // in turns, less the whole ones, before anything is rounded to f32: a position of a million costs no digits
+              double turns = static_cast<double>(position) * A.frequencies[i - t * half] * 0.15915494309189533577;
+              turns -= rint(turns);
+              float2 cs;
+              sincospif(2.0f * static_cast<float>(turns), &cs.y, &cs.x);
+              angles[i] = cs;
             }
-          } else if (at >= 0) {
-            const int64_t dst = at * C.page_stride + (static_cast<int64_t>(head) * P + kept + c0 + t) * D;
+          __syncthreads();
+          const float2* cs = half ? angles : nullptr;
+          for (int i = tid; !queries && i < m * units; i += kAppendThreads) {
+            const int t = i >> log_units;
+            const Piece u = piece_of(A, i & (units - 1));
+            const int64_t k_at = (row0 + c0 + t) * A.ld_k + head * D, v_at = (row0 + c0 + t) * A.ld_v + head * D;
+            float4 kx[2], vx[2];
+            const int64_t from_k[2] = {k_at + u.lo, k_at + u.hi}, from_v[2] = {v_at + u.lo, v_at + u.hi};
+            load_rows4(A.k, A.kv_dtype, from_k, A.k_vec, kx);
+            load_rows4(A.v, A.kv_dtype, from_v, A.v_vec, vx);
+            float x[8], y[8];
+            turn(A, kx[0], kx[1], u, half ? cs + t * half : nullptr, x);
+            turn(A, vx[0], vx[1], u, nullptr, y);
+            if (pass == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = now[0] == now[0] ? x[j] * inverse[0] : 0.0f, y[j] = now[1] == now[1] ? y[j] * inverse[1] : 0.0f;
-            *reinterpret_cast<uint32_t*>(C.k + dst + u.lo) = codes4(x, A.int8);
-            *reinterpret_cast<uint32_t*>(C.k + dst + u.hi) = codes4(x + 4, A.int8);
-            *reinterpret_cast<uint32_t*>(C.v + dst + u.lo) = codes4(y, A.int8);
-            *reinterpret_cast<uint32_t*>(C.v + dst + u.hi) = codes4(y + 4, A.int8);
-          }
-        }
-        if (queries) {  // two pieces of a thread on their way at once
-          const int all = m * A.group << log_units;
-          for (int i0 = tid; i0 < all; i0 += 2 * kAppendThreads) {
-            Piece u[2];
-            int token[2];
-            int64_t col[2], from[4];
-            float4 x[4];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int i = min(i0 + e * kAppendThreads, all - 1), r = i >> log_units;
-              token[e] = r / A.group;
-              u[e] = piece_of(A, i & (units - 1));
-              col[e] = static_cast<int64_t>(head * A.group + r - token[e] * A.group) * D;
-              const int64_t at = (row0 + c0 + token[e]) * A.ld_q + col[e];
-              from[2 * e] = at + u[e].lo, from[2 * e + 1] = at + u[e].hi;
-            }
-            load_rows4(A.q, A.q_dtype, from, A.q_vec, x);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if (i0 + e * kAppendThreads >= all) break;
-              float y[8];
-              turn(A, x[2 * e], x[2 * e + 1], u[e], half ? cs + token[e] * half : nullptr, y);
-              const int64_t at = (row0 + c0 + token[e]) * A.ld_q_out + col[e];
-              store4(A.q_out, A.q_out_dtype, at + u[e].lo, y, A.q_out_vec);
-              store4(A.q_out, A.q_out_dtype, at + u[e].hi, y + 4, A.q_out_vec);
-            }
-          }
-        }
-      }
-      if (pass == 0 && !queries) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          large[w] = __reduce_max_sync(0xffffffffu, large[w]);
-          if ((tid & 31) == 0) atomicMax(&most[w], large[w]);
-        }
-        __syncthreads();
-        if (at < 0) break;
-        const int64_t sc = static_cast<int64_t>(at) * C.kv_heads + head;
-        float* const scales[2] = {C.k_scale + sc, C.v_scale + sc};
-        uint8_t* const codes[2] = {C.k, C.v};
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const float want = scale_for(most[w], A.int8), was = kept ? *scales[w] : want;
-          // not-a-number, of old or of new values, stays
-          now[w] = was != was || want != want ? __uint_as_float(0x7fffffffu) : fmaxf(was, want);
-          inverse[w] = 1.0f / now[w];
-          if (kept && now[w] > was) {
-            const float ratio = was / now[w];
-            uint4* held = reinterpret_cast<uint4*>(codes[w] + at * C.page_stride + static_cast<int64_t>(head) * P * D);
-            for (int i = tid; i < kept * D / 16; i += kAppendThreads) {
-              const uint4 old = held[i];
-              uint32_t word[4] = {old.x, old.y, old.z, old.w};
-#pragma unroll
-              for (int b = 0; b < 4; ++b) {
-                float x[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const uint32_t code = word[b] >> (8 * j) & 0xffu;
-                  x[j] = (A.int8 ? static_cast<float>(static_cast<int8_t>(code)) : (code & 0x7fu) == 0x7fu ? __uint_as_float(0x7fffffffu) : e4m3_to_f32(code)) * ratio;
-                }
-                word[b] = codes4(x, A.int8);
+              for (int j = 0; j < 8; ++j) {
+                large[0] = max(large[0], __float_as_uint(x[j]) & 0x7fffffffu);  // as integers: not-a-number is the largest
+                large[1] = max(large[1], __float_as_uint(y[j]) & 0x7fffffffu);
               }
-              held[i] = make_uint4(word[0], word[1], word[2], word[3]);
+            } else if (at >= 0) {
+              const int64_t dst = at * C.page_stride + (static_cast<int64_t>(head) * P + kept + c0 + t) * D;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[j] = now[0] == now[0] ? x[j] * inverse[0] : 0.0f, y[j] = now[1] == now[1] ? y[j] * inverse[1] : 0.0f;
+              *reinterpret_cast<uint32_t*>(C.k + dst + u.lo) = codes4(x, A.int8);
+              *reinterpret_cast<uint32_t*>(C.k + dst + u.hi) = codes4(x + 4, A.int8);
+              *reinterpret_cast<uint32_t*>(C.v + dst + u.lo) = codes4(y, A.int8);
+              *reinterpret_cast<uint32_t*>(C.v + dst + u.hi) = codes4(y + 4, A.int8);
+            }
+          }
+          if (queries) {  // two pieces of a thread on their way at once
+            const int all = m * A.group << log_units;
+            for (int i0 = tid; i0 < all; i0 += 2 * kAppendThreads) {
+              Piece u[2];
+              int token[2];
+              int64_t col[2], from[4];
+              float4 x[4];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int i = min(i0 + e * kAppendThreads, all - 1), r = i >> log_units;
+                token[e] = r / A.group;
+                u[e] = piece_of(A, i & (units - 1));
+                col[e] = static_cast<int64_t>(head * A.group + r - token[e] * A.group) * D;
+                const int64_t at = (row0 + c0 + token[e]) * A.ld_q + col[e];
+                from[2 * e] = at + u[e].lo, from[2 * e + 1] = at + u[e].hi;
+              }
+              load_rows4(A.q, A.q_dtype, from, A.q_vec, x);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                if (i0 + e * kAppendThreads >= all) break;
+                float y[8];
+                turn(A, x[2 * e], x[2 * e + 1], u[e], half ? cs + token[e] * half : nullptr, y);
+                const int64_t at = (row0 + c0 + token[e]) * A.ld_q_out + col[e];
+                store4(A.q_out, A.q_out_dtype, at + u[e].lo, y, A.q_out_vec);
+                store4(A.q_out, A.q_out_dtype, at + u[e].hi, y + 4, A.q_out_vec);
+              }
             }
           }
         }
-        __syncthreads();  // every thread has read the old scales
-        if (tid < 2) *scales[tid] = now[tid];
+        if (pass == 0 && !queries) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            large[w] = __reduce_max_sync(0xffffffffu, large[w]);
+            if ((tid & 31) == 0) atomicMax(&most[w], large[w]);
+          }
+          __syncthreads();
+          if (at < 0) break;
+          const int64_t sc = static_cast<int64_t>(at) * C.kv_heads + head;
+          float* const scales[2] = {C.k_scale + sc, C.v_scale + sc};
+          uint8_t* const codes[2] = {C.k, C.v};
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const float want = scale_for(most[w], A.int8), was = kept ? *scales[w] : want;
+            // not-a-number, of old or of new values, stays
+            now[w] = was != was || want != want ? __uint_as_float(0x7fffffffu) : fmaxf(was, want);
+            inverse[w] = 1.0f / now[w];
+            if (kept && now[w] > was) {
+              const float ratio = was / now[w];
+              uint4* held = reinterpret_cast<uint4*>(codes[w] + at * C.page_stride + static_cast<int64_t>(head) * P * D);
+              for (int i = tid; i < kept * D / 16; i += kAppendThreads) {
+                const uint4 old = held[i];
+                uint32_t word[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                  float x[4];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    const uint32_t code = word[b] >> (8 * j) & 0xffu;
+                    x[j] = (A.int8 ? static_cast<float>(static_cast<int8_t>(code)) : (code & 0x7fu) == 0x7fu ? __uint_as_float(0x7fffffffu) : e4m3_to_f32(code)) * ratio;
+                  }
+                  word[b] = codes4(x, A.int8);
+                }
+                held[i] = make_uint4(word[0], word[1], word[2], word[3]);
+              }
+            }
+          }
+          __syncthreads();  // every thread has read the old scales
+          if (tid < 2) *scales[tid] = now[tid];
+        }
       }
     }
-    __syncthreads();  // before `most` starts anew
   }
+  if (x == 0 && blockIdx.y == 0)
+    for (int c = tid; c < C.sequences; c += kAppendThreads) {
+      bool bad;
+      const Span q = span_of(C, c, bad);
+      if (bad || q.length < q.n) report_batch(C);
+    }
 }
 
 // Whether rows of heads begin and go on in pieces of four values.
@@ -255,9 +278,11 @@ extern "C" int lx_b200_kv_append(const lx_b200_kv_cache* cache, const lx_b200_kv
   A.int8 = cache->type == LX_W_INT8;
   A.k_vec = fours(k, kv_dtype, ld_k), A.v_vec = fours(v, kv_dtype, ld_v), A.q_vec = fours(q, q_dtype, ld_q), A.q_out_vec = fours(q_out, q_out_dtype, ld_q_out);
   A.positions = positions, A.frequencies = frequencies;
-  // CTAs per sequence and head: as many pages as max_new tokens reach at most (a sequence with more: its CTAs take several)
-  const int P = cache->page_tokens, most = std::min(std::max(batch->max_new, 1), batch->tokens);
-  A.splits = (most + P - 2) / P + 1;
-  return launch_kernel(kv_append_kernel, dim3(static_cast<unsigned>(batch->sequences) * A.splits, static_cast<unsigned>(H) * (heads ? 2 : 1)), dim3(kAppendThreads), 0,
+  const int64_t places = batch->tokens / cache->page_tokens + 2 * static_cast<int64_t>(batch->sequences);
+  if (places > INT_MAX) return kNotSupported;
+  const int64_t splits = (std::min(std::max(batch->max_new, 1), batch->tokens) + cache->page_tokens - 2) / cache->page_tokens + 1;
+  const bool even = splits * batch->sequences <= places;
+  A.splits = even ? static_cast<int>(splits) : 0;
+  return launch_kernel(kv_append_kernel, dim3(static_cast<unsigned>(even ? splits * batch->sequences : places), static_cast<unsigned>(H) * (heads ? 2 : 1)), dim3(kAppendThreads), 0,
                        static_cast<cudaStream_t>(stream), A);
 }

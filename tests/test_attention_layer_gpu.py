@@ -186,7 +186,7 @@ def test_append_of_more_tokens_than_the_hint(lx):
     S = R.Sequences([70, 3], [75, 9], P, seed=3)
     x = normal((S.rows, K * D), 6)
     results = []
-    for hint in (1, 70, 0, 10**6):
+    for hint in (1, 70, 0, 10**6):  # both ways of cutting the work
         cache, _ = make_cache(lx, S, K, D, kind, 13)
         cache.append(put(S, max_new=hint), x.cuda(), x.cuda())
         results.append(torch.cat([cache.k.flatten(), cache.v.flatten(), cache.k_scale.flatten().view(torch.uint8)]).cpu())
