@@ -387,6 +387,54 @@ def test_attention_with_offsets_past_32_bits(lx):
     assert torch.equal(views[1].cpu(), want) and torch.equal(cache.v_scale.cpu(), scale)
 
 
+@pytest.mark.parametrize("n", [1, 60])
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 1.5])
+def test_attention_with_any_scale(lx, n, scale):
+    S = R.Sequences([n, 1], [n + 150, 77], 16, seed=12)
+    check_attention(lx, S, 2, 2, 128, "int8", scale=scale, spread=0.5)
+    check_attention(lx, S, 1, 4, 64, "fp8", scale=scale, spread=0.5, window=30, dtype=torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_that_begin_anywhere(lx, dtype):
+    """Odd offsets and strides of queries, keys, values and results: the same values as rows on 16 bytes."""
+    K, G, D, P = 2, 3, 64, 16
+    W, KV = K * G * D, K * D
+    for n in (1, 90):
+        S = R.Sequences([n, 2], [n + 50, 40], P, seed=13)
+        rows = normal((S.rows, W + 2 * KV), 14, dtype=dtype).cuda()
+        odd = torch.full((S.rows, W + 2 * KV + 5), 3.0, dtype=dtype, device="cuda")[:, 3:-2]
+        odd.copy_(rows)
+        caches = [make_cache(lx, S, K, D, "fp8", 15)[0] for _ in range(2)]
+        one = host.Rotary.of(32, device="cuda")
+        batch, outs = put(S), []
+        for cache, x in zip(caches, (rows, odd)):
+            q_out = torch.zeros((S.rows, W + 7), dtype=dtype, device="cuda")[:, 1:W + 1] if x is odd else torch.zeros((S.rows, W), dtype=dtype, device="cuda")
+            q = cache.append(batch, x[:, W:W + KV], x[:, W + KV:], q=x[:, :W], rotary=one, q_out=q_out)
+            out = torch.zeros((S.rows, W + 9), dtype=torch.bfloat16, device="cuda")[:, 5:W + 5] if x is odd else torch.zeros((S.rows, W), dtype=torch.bfloat16, device="cuda")
+            outs.append((q.clone(), host.Attention(cache, K * G)(batch, q, out=out).clone(), cache.k.clone(), cache.v.clone(), cache.k_scale.clone(), cache.v_scale.clone()))
+        util.check_status(lx)
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_many_sequences(lx):
+    """More sequences than a CTA has threads, some of them with many new tokens, some with none."""
+    g = torch.Generator().manual_seed(16)
+    total = torch.randint(1, 200, (333,), generator=g).tolist()
+    new = [0 if i % 7 == 3 else min(t, 40) if i % 50 == 0 else 1 for i, t in enumerate(total)]
+    S = R.Sequences(new, total, 16, seed=17, rows_behind=2)
+    check_attention(lx, S, 2, 4, 64, "fp8", max_new=1)
+    check_attention(lx, S, 2, 4, 64, "int8")
+    K, D = 2, 64
+    x = normal((S.rows, K * D), 18)
+    for hint in (1, 40):
+        cache, (k0, ks0, v0, vs0) = make_cache(lx, S, K, D, "int8", 19)
+        cache.append(put(S, max_new=hint), x.cuda(), x.cuda())
+        util.check_status(lx)
+        v, vs = R.append(v0, vs0, "int8", x.double().reshape(S.rows, K, D), S.starts, S.total, S.table, 16)
+        assert torch.equal(cache.v.cpu(), v) and torch.equal(cache.v_scale.cpu(), vs)
+
+
 # ---- norms -------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("T,C", [(1, 4096), (3, 8), (2, 1), (5, 1000), (33, 2048), (2, 8192), (3, 8200), (2, 16384), (2, 16392), (7, 4097), (300, 4096), (310, 5000), (300, 16384)])
 @pytest.mark.parametrize("y,h,w,gate,sigmoid,post,x", [
