@@ -114,11 +114,12 @@ def store_weight(lib: abi.Library, w_bf16: torch.Tensor, wtype: int) -> StoredWe
 
 
 class Linear:
-    """y = x @ W^T for one stored weight [N, K], choosing the entry point as the engine's linear() does."""
+    """y = x @ W^T for one stored weight [N, K], choosing the entry point as the engine's linear() does. Each call takes its workspace
+    from torch's allocator, so calls on several streams and captured graphs share none."""
 
     def __init__(self, lib: abi.Library, weight: StoredWeight, N: int, K: int):
         self.lib, self.weight, self.N, self.K = lib, weight, N, K
-        self._ws = None
+        self._need = {}  # bytes of workspace, by rows
 
     def __call__(self, x: torch.Tensor, y: torch.Tensor | None = None) -> torch.Tensor:
         """x: bf16 or f32 [M, K] on the device; y: f32 [M, N] (allocated when absent).
@@ -140,11 +141,14 @@ class Linear:
                 if st:
                     raise RuntimeError(f"lx_gemv_w failed: {st}")
             return y
-        need = self.lib.lx_gemm_workspace_bytes(M, K, abi.MATH_BF16)
-        if self._ws is None or self._ws.numel() < need:
-            self._ws = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)
+        need = self._need.get(M)
+        if need is None:
+            need = max(self.lib.lx_gemm_workspace_bytes(M, K, abi.MATH_BF16), 256)
+            if len(self._need) < 4096:
+                self._need[M] = need
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         st = self.lib.lx_gemm_w(x.data_ptr(), x_dt, ld_x, self.weight.ref(), abi.MATH_BF16, None, abi.BF16, y.data_ptr(), y_dt, ld_y, M, N, K, 1.0, 0.0,
-                                self._ws.data_ptr(), stream)
+                                ws.data_ptr(), stream)
         if st:
             raise RuntimeError(f"lx_gemm_w failed: {st}")
         return y
