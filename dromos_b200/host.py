@@ -192,11 +192,12 @@ class ShardedLinear:
 
 
 class Experts:
-    """Routed experts on stored stacks gate_up [E, 2I, L] and down [E, L, I] (lx_moe_route + lx_moe_experts_grouped)."""
+    """Routed experts on stored stacks gate_up [E, 2I, L] and down [E, L, I] (lx_moe_route + lx_moe_experts_grouped). Each call takes
+    its workspace from torch's allocator, as Linear's do."""
 
     def __init__(self, lib, gate_up: StoredWeight, down: StoredWeight, E: int, L: int, I: int, top_k: int):
         self.lib, self.gate_up, self.down, self.E, self.L, self.I, self.top_k = lib, gate_up, down, E, L, I, top_k
-        self._ws = None
+        self._need = {}  # bytes of workspace, by tokens
 
     def route(self, logits: torch.Tensor, bias: torch.Tensor | None = None):
         T = logits.shape[0]
@@ -216,11 +217,14 @@ class Experts:
         T = latent.shape[0]
         if out is None:
             out = torch.empty((T, self.L), dtype=torch.float32, device=latent.device)
-        need = self.lib.lx_moe_grouped_workspace_bytes(T, self.L, self.I, self.E, self.top_k, abi.MATH_BF16)
-        if self._ws is None or self._ws.numel() < need:
-            self._ws = torch.empty(need, dtype=torch.uint8, device=latent.device)
+        need = self._need.get(T)
+        if need is None:
+            need = self.lib.lx_moe_grouped_workspace_bytes(T, self.L, self.I, self.E, self.top_k, abi.MATH_BF16)
+            if len(self._need) < 4096:
+                self._need[T] = need
+        ws = torch.empty(need, dtype=torch.uint8, device=latent.device)
         st = self.lib.lx_moe_experts_grouped(latent.data_ptr(), ids.data_ptr(), weights.data_ptr(), self.gate_up.ref(), self.down.ref(), abi.MATH_BF16,
-                                             out.data_ptr(), self._ws.data_ptr(), T, self.L, self.I, self.E, self.top_k, _raw_stream())
+                                             out.data_ptr(), ws.data_ptr(), T, self.L, self.I, self.E, self.top_k, _raw_stream())
         if st:
             raise RuntimeError(f"lx_moe_experts_grouped failed: {st}")
         return out
@@ -784,7 +788,6 @@ class FusedShardedLinear:
         self._y_ptrs, self._c_ptrs = [int(p) for p in hy.buffer_ptrs], [int(p) for p in hc.buffer_ptrs]
         self._c_array = (ctypes.c_void_p * self.world)(*self._c_ptrs)
         self._calls, self._total = 0, {}
-        self._ws = None
         torch.cuda.synchronize()
         dist.barrier(self.group)
 
@@ -796,14 +799,12 @@ class FusedShardedLinear:
         self._calls += 1
         stride = self.max_rows * self.N * 4
         y_array = (ctypes.c_void_p * self.world)(*[p + half * stride for p in self._y_ptrs])
-        need = self.lib.lx_gemm_workspace_bytes(M, self.K, abi.MATH_BF16)
-        if self._ws is None or self._ws.numel() < need:
-            self._ws = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)
+        ws = torch.empty(max(self.lib.lx_gemm_workspace_bytes(M, self.K, abi.MATH_BF16), 256), dtype=torch.uint8, device=x.device)
         added = ctypes.c_int(0)
         x_dt = abi.BF16 if x.dtype == torch.bfloat16 else abi.F32
         st = self.lib.lx_b200_linear_allgather(abi.ptr(x), x_dt, x.stride(0), self.weight.ref(), None, abi.BF16, y_array, self._c_array,
                                                self.world, self.rank, self.n0, abi.F32, self.N, M, self.n1 - self.n0, self.K, 1.0,
-                                               abi.ptr(self._ws),
+                                               abi.ptr(ws),
                                                ctypes.byref(added), _stream())
         if st:
             raise RuntimeError(f"lx_b200_linear_allgather failed: {st}")
