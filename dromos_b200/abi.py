@@ -139,6 +139,7 @@ EXTENSIONS = {
                                   c_int, c_ptr]),
     # cache, batch, q, q_dtype, ld_q, q_heads, scale, window, out, ld_out, workspace, stream
     "lx_b200_attention": (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_f32, c_int, c_ptr, c_int, c_ptr, c_ptr]),
+    "lx_b200_attention_padded": (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_int, c_int, c_f32, c_int, c_ptr, c_int, c_ptr, c_ptr]),
     "lx_b200_attention_workspace_bytes": (c_i64, [c_ptr, c_ptr, c_int]),
     # y, y_dtype, ld_y, h, h_dtype, ld_h, gate, gate_dtype, ld_gate, gate_sigmoid, post, pre, weight_dtype, residual_scale, block_scale, eps, h_out, ld_h_out,
     # x, x_dtype, ld_x, T, C, stream

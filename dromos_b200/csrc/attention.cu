@@ -409,18 +409,35 @@ __global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stre
   }
 }
 
+// Zeros in the rows of no sequence, which begin at row `from`: all CTAs of a kernel, all of their threads.
+__device__ __forceinline__ void zero_rows_from(const AttentionArgs& A, int from, int head_dim) {
+  if (from < 0) return;
+  for (int64_t row = static_cast<int64_t>(from) + blockIdx.x; row < A.kv.tokens; row += gridDim.x)
+    for (int c = 4 * threadIdx.x; c < A.q_heads * head_dim; c += 4 * blockDim.x) store_out(A, row * A.ld_out + c, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f);
+}
+// The same by itself, for calls whose sequences all go to the tiles. (In the tiles' join it took 0.6 us of every call, asked for or not.)
+__global__ void __launch_bounds__(kThreads) attention_pad_kernel(const __grid_constant__ AttentionArgs A, int head_dim) {
+  pdl_wait();
+  zero_rows_from(A, A.kv.starts[A.kv.sequences], head_dim);
+}
+
 // Joins the units that several CTAs of the stream kernel shared: CTA i the one that began in share i and went on into the next. The
 // parts' maxima and sums are looked at 32 parts at once, a lane for each; their accumulators are read by as many groups of threads as
-// there are threads for (a part takes a thread 300 cycles, whatever is in flight beside it).
+// there are threads for (a part takes a thread 300 cycles, whatever is in flight beside it). As many CTAs as the stream kernel has are
+// resident at once (one more wave of CTAs that find nothing costs 0.8 us). The rows of no sequence are zeroed here where that is asked for.
 template <int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttentionArgs A) {
+__global__ void __launch_bounds__(kJoinThreads, stream_ctas<D, NT>()) attention_join_kernel(const __grid_constant__ AttentionArgs A) {
   constexpr int ROWS = 8 * NT, AT_ONCE = 32, CELLS = ROWS * (D / 4);  // four values each
   constexpr int GROUPS = CELLS >= kJoinThreads ? 1 : kJoinThreads / CELLS, ITEMS = CELLS > kJoinThreads ? CELLS / kJoinThreads : 1;
   __shared__ float ms[AT_ONCE][ROWS + 1], ls[AT_ONCE][ROWS + 1], shrink[ROWS], sums[ROWS], tops[ROWS];
   __shared__ float4 gathered[GROUPS > 1 ? GROUPS - 1 : 1][GROUPS > 1 ? CELLS : 1];
   pdl_wait();
   const JoinInfo u = A.join[blockIdx.x];
-  if (u.rows == 0) return;
+  const int behind = A.pad ? A.kv.starts[A.kv.sequences] : A.kv.tokens;  // on its way while the parts are joined
+  if (u.rows == 0) {
+    zero_rows_from(A, behind, D);
+    return;
+  }
   const int tid = threadIdx.x, first = blockIdx.x, group = GROUPS > 1 ? tid / CELLS : 0, cell0 = GROUPS > 1 ? tid % CELLS : tid;
   const int64_t slot_floats = ROWS * (D + 2);
   auto slot = [&](int p) { return A.partial + (2 * static_cast<int64_t>(p) + (p == first)) * slot_floats; };
@@ -461,6 +478,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
       }
     }
   }
+  zero_rows_from(A, behind, D);
   if constexpr (GROUPS > 1) {
     if (group > 0) gathered[group - 1][cell0] = v[0];
     __syncthreads();
@@ -550,15 +568,21 @@ extern "C" int64_t lx_b200_attention_workspace_bytes(const lx_b200_kv_cache* cac
   return attention_plan(*cache, *batch, q_heads / cache->kv_heads).total;
 }
 
-extern "C" int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q, int q_heads,
-                                 float scale, int window, void* out, int ld_out, void* workspace, void* stream) {
+static int attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q, int q_heads, float scale, int window,
+                     void* out, int ld_out, void* workspace, void* stream, bool pad) {
   if (int e = check_cache(cache)) return e;
   if (int e = check_batch(batch)) return e;
   const int64_t width = static_cast<int64_t>(q_heads) * cache->head_dim;
   if (!valid_dtype(q_dtype) || q_heads < 1 || q_heads % cache->kv_heads || window < 0 || width > INT_MAX) return kInvalid;
-  if (batch->sequences == 0 || batch->tokens == 0) return kOk;
+  if (batch->tokens == 0 || (batch->sequences == 0 && !pad)) return kOk;
   if (static_cast<int64_t>(batch->tokens) * (q_heads / cache->kv_heads) > INT_MAX / 2) return kNotSupported;
   if (!q || !out || ld_q < width || ld_out < width || !workspace || !aligned(workspace, 256)) return kInvalid;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (batch->sequences == 0) {
+    const cudaError_t e = cudaMemset2DAsync(out, static_cast<size_t>(ld_out) * 2, 0, static_cast<size_t>(width) * 2, static_cast<size_t>(batch->tokens), st);
+    if (e != cudaSuccess) cudaGetLastError();
+    return static_cast<int>(e);
+  }
   AttentionArgs A;
   A.kv = view_of(*cache, *batch);
   A.q = q, A.out = static_cast<uint16_t*>(out), A.ld_q = ld_q, A.ld_out = ld_out, A.partial = static_cast<float*>(workspace);
@@ -566,17 +590,27 @@ extern "C" int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv
   A.out_vec = aligned(out, 8) && ld_out % 4 == 0, A.q_vec = aligned(q, q_dtype == LX_BF16 ? 8 : 16) && ld_q % 4 == 0;
   A.scale_log2 = scale * 1.4426950408889634f;
   A.min_tiles = 3;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool int8 = cache->type == LX_W_INT8;
   const AttentionPlan plan = attention_plan(*cache, *batch, A.group);
   const int limit = stream_rows(cache->head_dim);
+  A.pad = pad;
   if (plan.tiles)
     if (int e = tile_attention(A, cache->head_dim, int8, limit, static_cast<uint8_t*>(workspace) + plan.tiles_at, st)) return e;
-  if (!plan.streams) return kOk;
+  if (!plan.streams) return pad ? launch_kernel(attention_pad_kernel, dim3(static_cast<unsigned>(std::min(batch->tokens, 4 * sm_count()))), dim3(kThreads), 0, st, A, cache->head_dim) : kOk;
   A.least = 1, A.most = plan.tiles ? limit : INT_MAX;
   switch (cache->head_dim) {
     case 64: return int8 ? stream_attention<true, 64>(A, plan.rows, st) : stream_attention<false, 64>(A, plan.rows, st);
     case 128: return int8 ? stream_attention<true, 128>(A, plan.rows, st) : stream_attention<false, 128>(A, plan.rows, st);
     default: return int8 ? stream_attention<true, 256>(A, plan.rows, st) : stream_attention<false, 256>(A, plan.rows, st);
   }
+}
+
+extern "C" int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q, int q_heads,
+                                 float scale, int window, void* out, int ld_out, void* workspace, void* stream) {
+  return attention(cache, batch, q, q_dtype, ld_q, q_heads, scale, window, out, ld_out, workspace, stream, false);
+}
+
+extern "C" int lx_b200_attention_padded(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q, int q_heads,
+                                        float scale, int window, void* out, int ld_out, void* workspace, void* stream) {
+  return attention(cache, batch, q, q_dtype, ld_q, q_heads, scale, window, out, ld_out, workspace, stream, true);
 }

@@ -21,6 +21,7 @@ struct AttentionArgs {
   int q_dtype, q_heads, group, window, min_tiles;
   float scale_log2;  // the softmax's scale times log2 e
   bool out_vec, q_vec;  // rows of `out` and of `q` go on in pieces of four values
+  bool pad;             // rows past the last sequence become zeros
   int least, most;   // the query rows per key head of the sequences that a kernel takes
 };
 

@@ -126,6 +126,7 @@ const Entry kEntries[] = {
     ENTRY(lx_moe_decode_workspace_bytes),
     ENTRY(lx_b200_kv_append),
     ENTRY(lx_b200_attention),
+    ENTRY(lx_b200_attention_padded),
     ENTRY(lx_b200_attention_workspace_bytes),
     ENTRY(lx_b200_norm_residual),
 };

@@ -328,7 +328,8 @@ class KvCache:
     def append(self, batch: KvBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, rotary: Rotary | None = None,
                positions: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
         """Writes the batch's new tokens, k and v [tokens, kv_heads * head_dim], to its pages, keys turned by `rotary`; returns the queries
-        q [tokens, heads * head_dim] turned the same way (bf16 where q_out does not say otherwise), None without q."""
+        q [tokens, heads * head_dim] turned the same way (bf16 where q_out does not say otherwise), None without q. Rows past the last
+        sequence are not written: in a result that is made here they hold anything."""
         T, width, device = batch.tokens, self.kv_heads * self.head_dim, self.device
         stream = _stream_on(device)
         if batch.device != device:
@@ -376,15 +377,17 @@ class Attention:
         self._need = {}  # bytes of workspace, by the sizes they go by
 
     def __call__(self, batch: KvBatch, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-        """q: f32 or bf16 [tokens, heads * head_dim]; out: bf16, the same shape (rows past the last sequence are left as they are)."""
+        """q: f32 or bf16 [tokens, heads * head_dim]; out: bf16, the same shape. Rows past the last sequence are left as they are; in a result
+        that is made here they are zeros."""
         cache, T, width = self.cache, batch.tokens, self.heads * self.cache.head_dim
         device, ld_o = cache.device, width
         stream = _stream_on(device)
         if batch.device != device:
             raise ValueError(f"the batch is on {batch.device}, the cache on {device}")
         ld_q, dt = _rows(q, T, width, "q", device), _dtype(q, "q")
+        attend = cache.lib.lx_b200_attention
         if out is None:
-            out = torch.empty((T, width), dtype=torch.bfloat16, device=device)
+            out, attend = torch.empty((T, width), dtype=torch.bfloat16, device=device), cache.lib.lx_b200_attention_padded
         elif out.dtype is not torch.bfloat16:
             raise TypeError("out: bfloat16")
         else:
@@ -397,8 +400,7 @@ class Attention:
             if len(self._need) < 4096:
                 self._need[batch.sizes] = need
         ws = torch.empty(need, dtype=torch.uint8, device=device)
-        st = cache.lib.lx_b200_attention(cache.address, batch.address, q.data_ptr(), dt, ld_q, self.heads, self.scale, self.window, out.data_ptr(), ld_o,
-                                         ws.data_ptr(), stream)
+        st = attend(cache.address, batch.address, q.data_ptr(), dt, ld_q, self.heads, self.scale, self.window, out.data_ptr(), ld_o, ws.data_ptr(), stream)
         if st:
             raise RuntimeError(f"lx_b200_attention failed: {st}")
         return out
@@ -476,7 +478,8 @@ class AttentionBlock:
             raise ValueError("the products' sizes are not those of the heads and the norm")
 
     def __call__(self, x: torch.Tensor, h: torch.Tensor, batch: KvBatch, positions: torch.Tensor | None = None, gate: torch.Tensor | None = None):
-        """x: the layer's input, normed, bf16 or f32 [tokens, K]; h: the residual stream. Returns what NormResidual returns."""
+        """x: the layer's input, normed, bf16 or f32 [tokens, K]; h: the residual stream. Returns what NormResidual returns; rows past the
+        last sequence are those of a layer whose attention gives zeros."""
         rows = self.qkv(x)
         width, kv = self.heads * self.cache.head_dim, self.cache.kv_heads * self.cache.head_dim
         q = self.cache.append(batch, rows[:, width:width + kv], rows[:, width + kv:], q=rows[:, :width], rotary=self.rotary, positions=positions)

@@ -339,6 +339,9 @@ LX_API int lx_b200_kv_append(const lx_b200_kv_cache* cache, const lx_b200_kv_bat
  * a sequence are cut to even out the work) and are the same every time. */
 LX_API int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q,
                              int q_heads, float scale, int window, void* out, int ld_out, void* workspace, void* stream);
+/* The same, and rows past starts[sequences] become zeros: for an `out` whose rows are all read on, whatever was in its memory. */
+LX_API int lx_b200_attention_padded(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q,
+                                    int q_heads, float scale, int window, void* out, int ld_out, void* workspace, void* stream);
 /* By the cache's head_dim and kv_heads, the batch's sequences, tokens and max_new (its device arrays are not looked at) and the current
  * device; -1 for arguments the call refuses. */
 LX_API int64_t lx_b200_attention_workspace_bytes(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, int q_heads);

@@ -6,8 +6,9 @@ import pytest
 import torch
 
 from dromos_b200 import abi, host
+from tests import kv_reference as R
 from tests import util
-from tests.test_attention_layer_gpu import make_block, normal
+from tests.test_attention_layer_gpu import make_block, make_cache, normal, put
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +74,46 @@ def test_one_block_on_two_streams(lx, wtype):
     util.check_status(lx)
     for all_of, w in zip(outs, want):
         assert all(torch.equal(a, b) for out in all_of for a, b in zip(out, w))
+
+
+def poison(mib=256):
+    """What the allocator hands out next holds not-a-number."""
+    blocks = [torch.full((n,), float("nan"), device="cuda") for n in [mib * 2**18] + [2**e for e in range(8, 21) for _ in range(4)]]
+    torch.cuda.synchronize()
+    del blocks
+
+
+# G, new tokens, hint: few rows, tiles beside few rows, tiles alone (a group of more heads than the kernel for few rows takes), no tokens at all
+PADDED = pytest.mark.parametrize("group,new,behind", [(4, [1, 1, 1], 2), (4, [1] * 20, 12), (4, [60, 1, 0, 7], 5), (40, [3, 1], 3), (4, [0, 0], 4), (4, [], 3), (4, [130], 1000)])
+
+
+@PADDED
+def test_rows_behind_the_last_sequence_are_zero_where_the_library_makes_the_results(lx, group, new, behind):
+    K, D, P = 2, 64, 16
+    S = R.Sequences(new, [n + 5 for n in new], P, seed=3, rows_behind=behind)
+    cache, _ = make_cache(lx, S, K, D, "fp8", 5)
+    q, attend = normal((S.rows, K * group * D), 6, dtype=torch.bfloat16).cuda(), host.Attention(cache, K * group)
+    poison()
+    out = attend(put(S), q)
+    util.check_status(lx)
+    assert bool((out[S.tokens:] == 0).all()) and bool(out.isfinite().all())
+    own = torch.full_like(out, 9.5)
+    assert attend(put(S), q, out=own) is own and torch.equal(own[:S.tokens], out[:S.tokens]) and bool((own[S.tokens:] == 9.5).all())
+
+
+@pytest.mark.parametrize("rows,behind", [(3, 2), (12, 4), (20, 44), (0, 6)])
+@pytest.mark.parametrize("wtype", [abi.W_BF16, abi.W_NVFP4], ids=["bf16", "nvfp4"])
+def test_a_padded_step(lx, rows, behind, wtype):
+    """A step of a fixed count of rows of which the last ones belong to no sequence: these get nothing from the block, whatever is in memory."""
+    block, _, _ = make_block(lx, "fp8", D, K, G, WIDTH, P, 100, wtype=wtype)
+    if rows:
+        decode_step(block, rows, 0, 50)
+    table = torch.arange(rows, dtype=torch.int32).reshape(rows, 1).cuda()
+    batch = host.KvBatch(int32(list(range(rows + 1))), int32([4] * rows), table, rows + behind, 1)
+    x, h = normal((rows + behind, WIDTH), 60).to(torch.bfloat16).cuda(), normal((rows + behind, WIDTH), 61).cuda()
+    poison()
+    got_h, got_x = block(x, h, batch)
+    util.check_status(lx)
+    want_h, want_x = block.norm(None, h[rows:])
+    assert torch.equal(got_h[rows:], want_h) and torch.equal(got_x[rows:], want_x)
+    assert bool(got_h.isfinite().all()) and bool(got_x.isfinite().all())
