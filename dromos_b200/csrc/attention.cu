@@ -31,7 +31,7 @@ __device__ __forceinline__ SeqWork work_of(const AttentionArgs& A, int s) {
   const int rows = w.q.n * A.group;
   w.blocks = rows <= A.most ? (rows + ROWS - 1) / ROWS : 0;
   const int first = w.q.length - w.q.n;
-  w.tile0 = A.window > 0 ? max(0, first - A.window + 1) / kTile : 0;
+  w.tile0 = first_seen(first + 1, A.window) / kTile;
   w.tiles = max(1, (w.q.length + kTile - 1) / kTile - w.tile0);
   w.all = static_cast<int64_t>(w.blocks) * A.kv.kv_heads * w.tiles;
   return w;
@@ -181,11 +181,11 @@ __global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stre
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * nt + 2 * t4 + e;
-        past[nt][e] = r < rows ? first + (row_block + r) / A.group + 1 : 0;
+        past[nt][e] = r < rows ? max(0, first + (row_block + r) / A.group + 1) : 0;
       }
     const int past_low = first + row_block / A.group + 1, past_high = first + (row_block + rows - 1) / A.group + 1;  // of the first and the last row
-    const int see_low = A.window > 0 ? max(0, past_low - A.window) : 0;                                              // the first slot that any row sees
-    const int see_all = A.window > 0 ? max(0, past_high - A.window) : 0;                                             // from here on all rows do
+    const int see_low = first_seen(past_low, A.window);   // the first slot that any row sees
+    const int see_all = first_seen(past_high, A.window);  // from here on all rows do
     float m[NT][2], l[NT][2], o[MT][NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {

@@ -27,6 +27,10 @@ struct AttentionArgs {
 
 namespace {
 
+// The first slot seen by a row that sees the slots before `past` (0 or less: none). `past` is as far below 0 as a
+// sequence is shorter than its new tokens, and a window as wide as an int: their difference need not be one.
+__device__ __forceinline__ int first_seen(int past, int window) { return window > 0 ? max(0, max(0, past) - window) : 0; }
+
 // 2^x, 2^-22 relative, results below f32's normal range 0.
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;

@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(1024) attention_plan_kernel(const __grid_const
         break;
       }
       const int r0 = b * C::kRows, r1 = min(rows, r0 + C::kRows) - 1;
-      const int low = A.window > 0 ? max(0, first + r0 / A.group + 1 - A.window) : 0, past = max(0, first + r1 / A.group + 1);
+      const int low = first_seen(first + r0 / A.group + 1, A.window), past = max(0, first + r1 / A.group + 1);
       const int tile0 = low / C::kKeys;
       T.plan[at + b] = {s0 + tid, r0, tile0, max(1, (past + C::kKeys - 1) / C::kKeys - tile0), 0};
     }
@@ -184,7 +184,7 @@ __device__ __forceinline__ bool next_part(const TileArgs& T, Share& w, Part& p) 
     p.rows = min(ROWS, p.q.n * A.group - b.row_block);
     const int first = p.q.length - p.q.n;
     p.past_high = max(0, first + (b.row_block + p.rows - 1) / A.group + 1);
-    p.see_low = A.window > 0 ? max(0, first + b.row_block / A.group + 1 - A.window) : 0;
+    p.see_low = first_seen(first + b.row_block / A.group + 1, A.window);
     return true;
   }
 }
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       const bool valid = r < p.row_block + p.rows;
       const int past = valid ? first + r / A.group + 1 : 0;
       const int past_low = first + row0 / A.group + 1, past_last = first + (min(row0 + kRowTile, p.row_block + p.rows) - 1) / A.group + 1;
-      const int see_all = A.window > 0 ? past_last - A.window : 0, low = A.window > 0 ? past - A.window : 0;
+      const int see_all = first_seen(past_last, A.window), low = first_seen(past, A.window);
       float m = -INFINITY, l = 0.0f;
       for (int i = 0; i < p.tiles; ++i) {
         const int key0 = (p.tile + i) * KT;
