@@ -32,7 +32,7 @@ __device__ __forceinline__ SeqWork work_of(const AttentionArgs& A, int s) {
   w.blocks = rows <= A.most ? (rows + ROWS - 1) / ROWS : 0;
   const int first = w.q.length - w.q.n;
   w.tile0 = first_seen(first + 1, A.window) / kTile;
-  w.tiles = max(1, (w.q.length + kTile - 1) / kTile - w.tile0);
+  w.tiles = max(1, tiles_before(w.q.length, kTile) - w.tile0);
   w.all = static_cast<int64_t>(w.blocks) * A.kv.kv_heads * w.tiles;
   return w;
 }
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stre
         const int r = 8 * nt + 2 * t4 + e;
         past[nt][e] = r < rows ? max(0, first + (row_block + r) / A.group + 1) : 0;
       }
-    const int past_low = first + row_block / A.group + 1, past_high = first + (row_block + rows - 1) / A.group + 1;  // of the first and the last row
+    const int past_low = max(0, first + row_block / A.group + 1), past_high = max(0, first + (row_block + rows - 1) / A.group + 1);  // of the first and the last row
     const int see_low = first_seen(past_low, A.window);   // the first slot that any row sees
     const int see_all = first_seen(past_high, A.window);  // from here on all rows do
     float m[NT][2], l[NT][2], o[MT][NT][4];
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stre
     // steps of 16 slots: this warp's every kWarps-th, those that some row sees
     int step = (W.tile0 + part0) * kWarps + warp;
     if (step < see_low / 16) step += (see_low / 16 - step + kWarps - 1) / kWarps * kWarps;
-    const int step_end = past_high <= 0 ? 0 : min((W.tile0 + part1) * kWarps, (past_high + 15) / 16);
+    const int step_end = min((W.tile0 + part1) * kWarps, tiles_before(past_high, 16));
     uint32_t kw[2][KW], vw[4][VW];
     auto page_at = [&](int st) {
       if (st >= step_end) return 0;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stre
       return p;
     };
     auto slot_base = [&](int page, int st) {
-      return max(page, 0) * C.page_stride + (static_cast<int64_t>(head) * C.page_tokens + (st * 16 & page_mask)) * D;
+      return max(page, 0) * C.page_stride + (static_cast<int64_t>(head) * C.page_tokens + (static_cast<uint32_t>(st) * 16 & page_mask)) * D;
     };
     auto load_k = [&](int64_t src) {
 #pragma unroll
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stre
       page = page_next;
       page_next = page_at(step + 2 * kWarps);
       const float v_scale = now.log_v < 0x1p-100f ? 0x1p-100f : now.log_v, log_v = __log2f(v_scale), inv_v = 0x1p-14f / v_scale;
-      const bool edge = slot + 16 > past_low || slot < see_all;
+      const bool edge = slot + 16u > static_cast<uint32_t>(past_low) || slot < see_all;
       bool higher = false;
       float shrink[NT][2];
 #pragma unroll
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stre
         p0[nt] = transpose8(*reinterpret_cast<const uint32_t*>(&a));
         p1[nt] = transpose8(*reinterpret_cast<const uint32_t*>(&b));
       }
-      if (slot + 16 > past_high || slot < see_low) {  // what no row sees may hold codes that are not numbers: 0 x NaN
+      if (slot + 16u > static_cast<uint32_t>(past_high) || slot < see_low) {  // what no row sees may hold codes that are not numbers: 0 x NaN
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int j = slot + 2 * t4 + (i & 1) + 8 * (i >> 1);

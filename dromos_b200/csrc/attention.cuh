@@ -30,6 +30,8 @@ namespace {
 // The first slot seen by a row that sees the slots before `past` (0 or less: none). `past` is as far below 0 as a
 // sequence is shorter than its new tokens, and a window as wide as an int: their difference need not be one.
 __device__ __forceinline__ int first_seen(int past, int window) { return window > 0 ? max(0, max(0, past) - window) : 0; }
+// Tiles that hold the slots before `past`, which may be the largest int: such sums are unsigned, here and where slots are compared with it.
+__device__ __forceinline__ int tiles_before(int past, int tile) { return past <= 0 ? 0 : static_cast<int>((static_cast<uint32_t>(past) + tile - 1) / tile); }
 
 // 2^x, 2^-22 relative, results below f32's normal range 0.
 __device__ __forceinline__ float exp2_fast(float x) {

@@ -119,9 +119,9 @@ __global__ void __launch_bounds__(1024) attention_plan_kernel(const __grid_const
         break;
       }
       const int r0 = b * C::kRows, r1 = min(rows, r0 + C::kRows) - 1;
-      const int low = first_seen(first + r0 / A.group + 1, A.window), past = max(0, first + r1 / A.group + 1);
+      const int low = first_seen(first + r0 / A.group + 1, A.window), past = first + r1 / A.group + 1;
       const int tile0 = low / C::kKeys;
-      T.plan[at + b] = {s0 + tid, r0, tile0, max(1, (past + C::kKeys - 1) / C::kKeys - tile0), 0};
+      T.plan[at + b] = {s0 + tid, r0, tile0, max(1, tiles_before(past, C::kKeys) - tile0), 0};
     }
     base += all;
   }
@@ -573,9 +573,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       bool ok = true;
       while (ok && next_part<C::kRows>(T, share, p)) {
         for (int i = 0; i < p.tiles && ok; ++i, ++n) {
-          const int slot = (p.tile + i) * KT + 16 * lane;
+          const int slot = (p.tile + i) * KT + 16 * (lane & (C::kScaleGroups - 1));
           int page = -2;  // nothing that any row sees
-          if (lane < C::kScaleGroups && slot < p.past_high && slot + 16 > p.see_low) {
+          if (lane < C::kScaleGroups && slot < p.past_high && slot > p.see_low - 16) {
             page = page_of(V, p.s, slot >> log_p);
             if (page < 0) report_batch(V);
           }
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         }
         ++sn;
         tc_fence_after();
-        const bool edge = key0 + KT > past_low || key0 < see_all;
+        const bool edge = key0 > past_low - KT || key0 < see_all;
         const int lo = low - key0, hi = past - key0;
         const float top = edge ? tile_top<true, KT>(s_tmem, sc, f_now, lo, hi) : tile_top<false, KT>(s_tmem, sc, f_now, lo, hi);
         const bool higher = top > m + kSlack;  // at first m is -inf
@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           ok = false;
           break;
         }
-        bool edge = slot0 < p.see_low || slot0 + KT > p.past_high;
+        bool edge = slot0 < p.see_low || slot0 > p.past_high - KT;
 #pragma unroll
         for (int g = 0; g < C::kScaleGroups; ++g) edge |= sc[g].w == 0.0f;
         {

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const __gr
     if (bad || q.length < q.n || q.n == 0) continue;
     const int first = q.length - q.n, place = A.splits > 0 ? x % A.splits : x - places_before(C, s), stride = A.splits > 0 ? A.splits : INT_MAX / 2;
     for (int page = first / P + place; page <= (q.length - 1) / P; page += stride) {
-      const int lo = max(first, page * P), n = min(q.length, page * P + P) - lo, row0 = q.row0 + lo - first, kept = lo - page * P;
+      const int lo = max(first, page * P), kept = lo - page * P, n = min(q.length - lo, P - kept), row0 = q.row0 + lo - first;
       const int at = page_of(C, s, page);
       if (at < 0 && tid == 0 && blockIdx.y == 0) report_batch(C);
       if (tid < 2) most[tid] = 0;
