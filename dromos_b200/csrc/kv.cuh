@@ -89,6 +89,7 @@ inline int check_cache(const lx_b200_kv_cache* c) {
 }
 inline int check_batch(const lx_b200_kv_batch* b) {
   if (!b || b->sequences < 0 || b->tokens < 0 || b->max_new < 0 || b->ld_pages < 0) return kInvalid;
+  if (b->sequences > (1 << 30)) return kNotSupported;  // loops over them count past the last one, in 32 bits
   if (b->sequences > 0 && (!b->starts || !b->lengths || (b->ld_pages > 0 && !b->pages))) return kInvalid;
   return kOk;
 }

@@ -1,9 +1,9 @@
-"""What lx_b200_attention_padded refuses: what lx_b200_attention does. No call here reaches a launch."""
+"""What lx_b200_attention_padded refuses: what lx_b200_attention does; and what no batch can hold. No call here reaches a launch."""
 
 import pytest
 
 from dromos_b200 import abi
-from tests.test_attention_layer_cpu import BAD_BATCHES, BAD_CACHES, UNSUPPORTED_CACHES, attend, batch, cache
+from tests.test_attention_layer_cpu import BAD_BATCHES, BAD_CACHES, UNSUPPORTED_CACHES, address, append, attend, batch, cache
 
 
 class Padded:
@@ -30,3 +30,12 @@ def test_padded_attentions_that_are_refused(lib):
         for kw in (dict(q=None), dict(out=None), dict(ld_q=255), dict(ld_out=255), dict(q_dtype=2), dict(q_heads=0), dict(q_heads=5), dict(window=-1), dict(workspace=None),
                    dict(workspace=4096 + 128)):
             assert attend(lib, cache(), b, **kw) == abi.ERR_INVALID, kw
+
+
+@pytest.mark.parametrize("sequences", [2**30 + 1, 2**31 - 128, 2**31 - 1])
+def test_more_sequences_than_the_kernels_count(sequences):
+    """Their loops over sequences count in steps of a CTA's threads, in 32 bits, and the order of work has a place for each."""
+    lib, b = abi.Library(abi.default_library_path()), batch(tokens=4, sequences=sequences)
+    assert attend(lib, cache(), b) == abi.ERR_NOT_SUPPORTED and attend(Padded(), cache(), b) == abi.ERR_NOT_SUPPORTED
+    assert append(lib, cache(), b) == abi.ERR_NOT_SUPPORTED
+    assert lib.lx_b200_attention_workspace_bytes(address(cache()), address(b), 4) == -1
