@@ -6,7 +6,8 @@
 // A row is one CTA's; a thread keeps its values in registers from the one read of y, h and gate to the writes of h' and x. Few rows are
 // a chain of latencies: all loads, the weights' among them, are issued at once (one row of 4096: 2.8 us). Many rows are bound by HBM,
 // and what counts is that one row of an SM loads while another one is summed: then the weights, which the caches hold, are read
-// where they are used, so that two CTAs of 512 threads fit the SM's registers. The same threads have the same values either way.
+// where they are used, so that two CTAs of 512 threads fit the SM's registers. The same threads have the same values either way, and
+// every product and sum of a value is written out, so that the compiler does not round once here and twice there.
 #include <algorithm>
 
 #include "launch.cuh"
@@ -105,23 +106,23 @@ __global__ void __launch_bounds__(512, LATE ? (PIECES == 1 ? 3 : PIECES == 2 ? 2
     float u[8], v[8];
     values_of(h[i], A.h_dtype, next[i]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) next[i][j] *= A.residual_scale;
+    for (int j = 0; j < 8; ++j) next[i][j] = __fmul_rn(next[i][j], A.residual_scale);
     if (A.y) {
       values_of(y[i], A.y_dtype, u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] *= scale;
+      for (int j = 0; j < 8; ++j) u[j] = __fmul_rn(u[j], scale);
       if (A.post) {
         values_of(LATE ? load_raw8(A.post, A.weight_dtype, 8 * p) : wp[LATE ? 0 : i], A.weight_dtype, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] *= v[j];
+        for (int j = 0; j < 8; ++j) u[j] = __fmul_rn(u[j], v[j]);
       }
       if (A.gate) {
         values_of(LATE ? load_raw8(A.gate, A.gate_dtype, row * A.ld_gate + 8 * p) : g[LATE ? 0 : i], A.gate_dtype, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] *= gate_of(v[j], A.gate_sigmoid);
+        for (int j = 0; j < 8; ++j) u[j] = __fmul_rn(u[j], gate_of(v[j], A.gate_sigmoid));
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) next[i][j] += u[j];
+      for (int j = 0; j < 8; ++j) next[i][j] = __fadd_rn(next[i][j], u[j]);
     }
     if (A.h_out) store8(A.h_out, A.h_dtype, row * A.ld_h_out + 8 * p, next[i]);
 #pragma unroll
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(512, LATE ? (PIECES == 1 ? 3 : PIECES == 2 ? 2
     float v[8];
     values_of(LATE ? load_raw8(A.pre, A.weight_dtype, 8 * p) : wn[LATE ? 0 : i], A.weight_dtype, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= next[i][j] * rms;
+    for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], __fmul_rn(next[i][j], rms));
     store8(A.x, A.x_dtype, row * A.ld_x + 8 * p, v);
   }
 }
