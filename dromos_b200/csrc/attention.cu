@@ -99,14 +99,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
+// Plain loads, not those of the read-only path: the kernel may be resident before the append that wrote the codes has ended.
 template <int WORDS>
 __device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t (&w)[WORDS]) {
   if constexpr (WORDS == 2) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
   } else {
 #pragma unroll
     for (int i = 0; i < WORDS; i += 4)
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "l"(p + 4 * i));
+      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "l"(p + 4 * i));
   }
 }
 

@@ -117,3 +117,32 @@ def test_a_padded_step(lx, rows, behind, wtype):
     want_h, want_x = block.norm(None, h[rows:])
     assert torch.equal(got_h[rows:], want_h) and torch.equal(got_x[rows:], want_x)
     assert bool(got_h.isfinite().all()) and bool(got_x.isfinite().all())
+
+
+@pytest.mark.parametrize("new", [1, 4, 24])
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+def test_attention_right_behind_appends_to_what_it_reads(lx, kind, new):
+    """Steps back to back on one stream, whose kernels may be resident before the last one has ended, and with a wait between any two calls:
+    the same codes, scales and results. Louder and louder tokens, so that appends rewrite the codes that the step before has read."""
+    S, steps, heads = 8, 30, K * G
+    table = torch.randperm(8 * 48, generator=torch.Generator().manual_seed(3)).to(torch.int32).reshape(8, 48).cuda()
+    starts, T = int32([new * i for i in range(S + 1)]), S * new
+    rows = [(normal((T, (heads + 2 * K) * D), 100 + i) * 1.2**i).cuda() for i in range(steps)]
+    lengths = [int32([new * (i + 1) + s for s in range(S)]) for i in range(steps)]
+    results = []
+    for wait in (False, True):
+        cache = host.KvCache.empty(lx, {"fp8": abi.W_FP8, "int8": abi.W_INT8}[kind], 8 * 48, K, D, P)
+        attend, turn, outs = host.Attention(cache, heads), host.Rotary.of(D, device="cuda"), []
+        torch.cuda.synchronize()
+        for i in range(steps):
+            batch, x = host.KvBatch(starts, lengths[i], table, T, new), rows[i]
+            q = cache.append(batch, x[:, heads * D:(heads + K) * D], x[:, (heads + K) * D:], q=x[:, :heads * D], rotary=turn)
+            if wait:
+                torch.cuda.synchronize()
+            outs.append(attend(batch, q))
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        util.check_status(lx)
+        results.append([torch.stack(outs), cache.k, cache.v, cache.k_scale, cache.v_scale])
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and bool(results[0][0].isfinite().all())
