@@ -298,7 +298,9 @@ LX_API void* lx_b200_moe_static_scratch_ptr(void);
  * A paged cache of keys and values in 8 bits. Pages of page_tokens slots (16, 32, 64 or 128); k and v hold, page_stride
  * bytes from one page to the next (a multiple of 16, the buffers on 16 bytes), codes [kv_heads][page_tokens][head_dim],
  * E4M3 (LX_W_FP8) or signed bytes (LX_W_INT8); head_dim 64, 128 or 256. A value is code * scale, one f32 scale, 0 or
- * more, per page and head: k_scale, v_scale [pages][kv_heads]. A host struct of device pointers, like lx_weight. */
+ * more, per page and head: k_scale, v_scale [pages][kv_heads]. The append writes no E4M3 code for not-a-number and no scale
+ * below 2^-100; attention may spread such a code of one token over rows that do not see it, and reads smaller scales of V as
+ * 2^-100. A host struct of device pointers, like lx_weight. */
 typedef struct {
   lx_wtype type;
   int32_t kv_heads, head_dim, page_tokens;
@@ -311,7 +313,8 @@ typedef struct {
  * sequence is slot i % page_tokens of page pages[s * ld_pages + i / page_tokens]. `tokens` rows are there in all: rows past
  * starts[sequences] are left as they are. max_new: the most new tokens of one sequence, as far as the host knows; it chooses
  * how the work is cut, a sequence with more is still computed. What the device arrays say is checked by the kernels: rows
- * outside the buffers, a page outside the cache or a sequence shorter than its new tokens shows as 9 in lx_b200_last_error. */
+ * outside the buffers or a page outside the cache show as 9 in lx_b200_last_error, and so does a sequence shorter than its new
+ * tokens where it is appended (attention takes it as it is: the tokens before slot 0 see nothing). At most 2^30 sequences. */
 typedef struct {
   int32_t sequences, tokens, max_new, ld_pages;
   const int32_t *starts, *lengths, *pages;
@@ -325,7 +328,8 @@ typedef struct {
  * or less. It starts anew when the page's first slot is written; when a later token needs a larger one, the codes the page holds are
  * rounded to it. Codes are rounded to nearest even. Values that are not finite make the page's scale of that head NaN, with codes
  * of 0, until its first slot is written again: all of that page and head then reads as NaN. No two sequences of a call may write
- * to one page. A sequence shorter than its new tokens, and tokens on a page outside the cache, are not written. */
+ * to one page, nor a sequence to one that its table has twice. A sequence shorter than its new tokens, and tokens on a page outside
+ * the cache, are not written. */
 LX_API int lx_b200_kv_append(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* k, int ld_k, const void* v,
                              int ld_v, lx_dtype kv_dtype, const void* q, lx_dtype q_dtype, int ld_q, int q_heads, void* q_out,
                              lx_dtype q_out_dtype, int ld_q_out, const int32_t* positions, const double* frequencies, int rotary_dim,
@@ -334,9 +338,11 @@ LX_API int lx_b200_kv_append(const lx_b200_kv_cache* cache, const lx_b200_kv_bat
  * head h / (q_heads / kv_heads) of the slots j <= p, with window > 0 of the last `window` of these (itself counted), and
  * out = sum_j softmax_j(scale * q . k_j) v_j. q: rows of q_heads * head_dim, f32 or bf16; out the same in bf16; a query that sees no slot
  * gets zeros. What unused slots and the table past a sequence's end hold is not read into any result; a page outside the
- * cache makes the rows that see it NaN. f32 sums and statistics. workspace: lx_b200_attention_workspace_bytes, 256-byte aligned,
- * what it holds does not matter; calls that may overlap need one each. A row's bits depend on the batch it is in (the keys of
- * a sequence are cut to even out the work) and are the same every time. */
+ * cache makes the rows that see it NaN. Both products have f16 operands and f32 sums: codes as they are; queries times a power of two
+ * that brings the row's largest below 2^15 (those in bf16 keep their bits down to 2^-31 of it, those in f32 keep 11); weights,
+ * 11 bits. Scales, maxima and sums of weights are f32. workspace: lx_b200_attention_workspace_bytes, 256-byte aligned, what it
+ * holds does not matter; calls that may overlap need one each. A row's bits depend on the batch it is in (the keys of a sequence
+ * are cut to even out the work) and are the same every time. */
 LX_API int lx_b200_attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batch, const void* q, lx_dtype q_dtype, int ld_q,
                              int q_heads, float scale, int window, void* out, int ld_out, void* workspace, void* stream);
 /* The same, and rows past starts[sequences] become zeros: for an `out` whose rows are all read on, whatever was in its memory. */
