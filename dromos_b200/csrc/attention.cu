@@ -113,16 +113,15 @@ __device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t (&w)[WORDS
 
 // What a warp needs of a step's page beside its codes.
 struct StepScale {
-  float k, log_v, inv_v;
+  float k, v;
 };
 __device__ __forceinline__ StepScale step_scale(const AttentionArgs& A, int page, int head) {
   if (page < 0) {
     const float nan = __uint_as_float(0x7fffffffu);
-    return {nan, nan, nan};
+    return {nan, nan};
   }
   const int64_t at = static_cast<int64_t>(page) * A.kv.kv_heads + head;
-  const float v = A.kv.v_scale[at];
-  return {A.kv.k_scale[at], v, 0.0f};
+  return {A.kv.k_scale[at], A.kv.v_scale[at]};
 }
 
 // CTAs of an SM: what the accumulators' registers leave room for. (256 values per head: three CTAs spill, 24 sequences 45 us for 43.)
@@ -217,7 +216,8 @@ __global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stre
 #pragma unroll
       for (int i = 0; i < 4; ++i) load_codes(C.v + src + (2 * t4 + (i & 1) + 8 * (i >> 1)) * D + g * (D / 8), vw[i]);
     };
-    int page = page_at(step), page_next = page_at(step + kWarps);
+    const int page = page_at(step);
+    int page_next = page_at(step + kWarps);
     // queries, while the table is read: each row times the power of two that brings it into f16's range
     {
       constexpr int PIECES = (D + 127) / 128, PER_WARP = ROWS / kWarps;
@@ -284,9 +284,8 @@ __global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stre
         load_k(src_next);
         sc = step_scale(A, page_next, head);
       }
-      page = page_next;
       page_next = page_at(step + 2 * kWarps);
-      const float v_scale = now.log_v < 0x1p-100f ? 0x1p-100f : now.log_v, log_v = __log2f(v_scale), inv_v = 0x1p-14f / v_scale;
+      const float v_scale = now.v < 0x1p-100f ? 0x1p-100f : now.v, log_v = __log2f(v_scale), inv_v = 0x1p-14f / v_scale;
       const bool edge = slot + 16u > static_cast<uint32_t>(past_low) || slot < see_all;
       bool higher = false;
       float shrink[NT][2];
@@ -598,7 +597,7 @@ static int attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batc
   if (plan.tiles)
     if (int e = tile_attention(A, cache->head_dim, int8, limit, static_cast<uint8_t*>(workspace) + plan.tiles_at, st)) return e;
   if (!plan.streams) return pad ? launch_kernel(attention_pad_kernel, dim3(static_cast<unsigned>(std::min(batch->tokens, 4 * sm_count()))), dim3(kThreads), 0, st, A, cache->head_dim) : kOk;
-  A.least = 1, A.most = plan.tiles ? limit : INT_MAX;
+  A.most = plan.tiles ? limit : INT_MAX;
   switch (cache->head_dim) {
     case 64: return int8 ? stream_attention<true, 64>(A, plan.rows, st) : stream_attention<false, 64>(A, plan.rows, st);
     case 128: return int8 ? stream_attention<true, 128>(A, plan.rows, st) : stream_attention<false, 128>(A, plan.rows, st);

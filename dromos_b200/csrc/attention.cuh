@@ -22,7 +22,7 @@ struct AttentionArgs {
   float scale_log2;  // the softmax's scale times log2 e
   bool out_vec, q_vec;  // rows of `out` and of `q` go on in pieces of four values
   bool pad;             // rows past the last sequence become zeros
-  int least, most;   // the query rows per key head of the sequences that a kernel takes
+  int most;             // the query rows per key head up to which a sequence is the stream kernel's; the tiles take those with more
 };
 
 namespace {

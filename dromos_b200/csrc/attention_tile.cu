@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(1024) attention_plan_kernel(const __grid_const
       rows = q.n * A.group;
       if (bad) report_batch(A.kv);
     }
-    const int blocks = rows >= A.least && rows <= A.most ? (rows + C::kRows - 1) / C::kRows : 0;
+    const int blocks = rows > A.most ? (rows + C::kRows - 1) / C::kRows : 0;
     int64_t all;
     const int64_t at = base + scan(blocks, all);
     const int first = q.length - q.n;
@@ -947,7 +947,7 @@ int tile_attention(AttentionArgs A, int head_dim, bool int8, int limit, void* wo
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   TileArgs T;
   T.a = A;
-  T.a.least = limit + 1, T.a.most = INT_MAX;
+  T.a.most = limit;
   T.a.min_tiles = 2 * kBlockCost + 2;
   T.header = reinterpret_cast<PlanHeader*>(ws), T.plan = reinterpret_cast<BlockPlan*>(ws + L.plan), T.partial = reinterpret_cast<float*>(ws + L.partial);
   T.capacity = L.capacity;

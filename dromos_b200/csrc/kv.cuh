@@ -19,8 +19,10 @@ struct KvView {
 
 namespace {
 
-// Smallest and largest exponent of a scale the append writes. The lower end keeps the sum of a softmax's weights, which are
-// held divided by these scales, inside f32: 2^100 times a million tokens is 2^120. No f32 needs one above the upper end.
+// Smallest and largest exponent of a scale the append writes. The lower end is for the sum of a softmax's weights, which are held divided
+// by these scales: at most 2^100 for a key where few rows are attended (2^120 for a million of them, inside f32), 2^108 where many are (the
+// weights' 2^15, less 2^7), whose sums pass f32 with a million keys that are all next to the lower end, such as values of zeros: the
+// results are then 0 for numbers below 2^-91. No f32 needs a scale above the upper end.
 constexpr int kScaleMin = -100, kScaleMax = 122;
 
 // A sequence's rows and slots, 0 new tokens where what the arrays say cannot be.

@@ -10,7 +10,7 @@
 // every product and sum of a value is written out, so that the compiler does not round once here and twice there.
 #include <algorithm>
 
-#include "launch.cuh"
+#include "tc.cuh"
 
 namespace b200 {
 namespace {
@@ -206,7 +206,7 @@ extern "C" int lx_b200_norm_residual(const void* y, lx_dtype y_dtype, int ld_y, 
   const bool pieces = C % 8 == 0 && whole(y, y_dtype, ld_y) && whole(h, h_dtype, ld_h) && whole(gate, gate_dtype, ld_gate) && whole(post, weight_dtype, 0) &&
                       whole(pre, weight_dtype, 0) && whole(h_out, h_dtype, ld_h_out) && whole(pre ? x : nullptr, x_dtype, ld_x);
   // how a row is dealt to threads goes by C alone, so a row's bits do not depend on the other rows
-  const bool late = T > 296;  // two rows for each SM: from here on rows wait for one another and not for their own loads
+  const bool late = T > 2 * sm_count();  // two rows for each SM: from here on rows wait for one another and not for their own loads
   auto threads = [&](int per) { return dim3(((C / 8 + per - 1) / per + 31) / 32 * 32); };
   if (pieces && C <= 8 * 512) return launch_kernel(late ? norm_kernel<1, true> : norm_kernel<1, false>, dim3(T), threads(1), 0, s, A);
   if (pieces && C <= 16 * 512) return launch_kernel(late ? norm_kernel<2, true> : norm_kernel<2, false>, dim3(T), threads(2), 0, s, A);
