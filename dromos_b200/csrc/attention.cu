@@ -409,18 +409,6 @@ __global__ void __launch_bounds__(kThreads, stream_ctas<D, NT>()) attention_stre
   }
 }
 
-// Zeros in the rows of no sequence, which begin at row `from`: all CTAs of a kernel, all of their threads.
-__device__ __forceinline__ void zero_rows_from(const AttentionArgs& A, int from, int head_dim) {
-  if (from < 0) return;
-  for (int64_t row = static_cast<int64_t>(from) + blockIdx.x; row < A.kv.tokens; row += gridDim.x)
-    for (int c = 4 * threadIdx.x; c < A.q_heads * head_dim; c += 4 * blockDim.x) store_out(A, row * A.ld_out + c, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f);
-}
-// The same by itself, for calls whose sequences all go to the tiles. (In the tiles' join it took 0.6 us of every call, asked for or not.)
-__global__ void __launch_bounds__(kThreads) attention_pad_kernel(const __grid_constant__ AttentionArgs A, int head_dim) {
-  pdl_wait();
-  zero_rows_from(A, A.kv.starts[A.kv.sequences], head_dim);
-}
-
 // Joins the units that several CTAs of the stream kernel shared: CTA i the one that began in share i and went on into the next. The
 // parts' maxima and sums are looked at 32 parts at once, a lane for each; their accumulators are read by as many groups of threads as
 // there are threads for (a part takes a thread 300 cycles, whatever is in flight beside it). As many CTAs as the stream kernel has are
@@ -435,7 +423,7 @@ __global__ void __launch_bounds__(kJoinThreads, stream_ctas<D, NT>()) attention_
   const JoinInfo u = A.join[blockIdx.x];
   const int behind = A.pad ? A.kv.starts[A.kv.sequences] : A.kv.tokens;  // on its way while the parts are joined
   if (u.rows == 0) {
-    zero_rows_from(A, behind, D);
+    zero_rows_from(A, behind, D, blockIdx.x, gridDim.x);
     return;
   }
   const int tid = threadIdx.x, first = blockIdx.x, group = GROUPS > 1 ? tid / CELLS : 0, cell0 = GROUPS > 1 ? tid % CELLS : tid;
@@ -478,7 +466,7 @@ __global__ void __launch_bounds__(kJoinThreads, stream_ctas<D, NT>()) attention_
       }
     }
   }
-  zero_rows_from(A, behind, D);
+  zero_rows_from(A, behind, D, blockIdx.x, gridDim.x);
   if constexpr (GROUPS > 1) {
     if (group > 0) gathered[group - 1][cell0] = v[0];
     __syncthreads();
@@ -593,10 +581,11 @@ static int attention(const lx_b200_kv_cache* cache, const lx_b200_kv_batch* batc
   const bool int8 = cache->type == LX_W_INT8;
   const AttentionPlan plan = attention_plan(*cache, *batch, A.group);
   const int limit = stream_rows(cache->head_dim);
-  A.pad = pad;
+  A.pad = pad && !plan.streams;  // by the last join of the call
   if (plan.tiles)
     if (int e = tile_attention(A, cache->head_dim, int8, limit, static_cast<uint8_t*>(workspace) + plan.tiles_at, st)) return e;
-  if (!plan.streams) return pad ? launch_kernel(attention_pad_kernel, dim3(static_cast<unsigned>(std::min(batch->tokens, 4 * sm_count()))), dim3(kThreads), 0, st, A, cache->head_dim) : kOk;
+  if (!plan.streams) return kOk;
+  A.pad = pad;
   A.most = plan.tiles ? limit : INT_MAX;
   switch (cache->head_dim) {
     case 64: return int8 ? stream_attention<true, 64>(A, plan.rows, st) : stream_attention<false, 64>(A, plan.rows, st);

@@ -52,6 +52,13 @@ __device__ __forceinline__ void store_out(const AttentionArgs& A, int64_t at, co
   }
 }
 
+// Zeros in the rows of no sequence, which begin at row `from`: all threads of a CTA, one of `ctas`.
+__device__ __forceinline__ void zero_rows_from(const AttentionArgs& A, int from, int head_dim, int cta, int ctas) {
+  if (from < 0) return;
+  for (int64_t row = static_cast<int64_t>(from) + cta; row < A.kv.tokens; row += ctas)
+    for (int c = 4 * threadIdx.x; c < A.q_heads * head_dim; c += 4 * blockDim.x) store_out(A, row * A.ld_out + c, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f);
+}
+
 // ---- codes to f16 pairs, exact ------------------------------------------------------------------------------------------
 template <bool kInt8>
 __device__ __forceinline__ void halves(uint32_t w, uint32_t& lo, uint32_t& hi) {  // codes 0, 1 and codes 2, 3

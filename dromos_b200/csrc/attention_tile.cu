@@ -877,6 +877,7 @@ __global__ void __launch_bounds__(256) attention_tile_join_kernel(const __grid_c
   pdl_wait();
   const AttentionArgs& A = T.a;
   const PlanHeader h = *T.header;
+  if (A.pad) zero_rows_from(A, A.kv.starts[A.kv.sequences], D, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
   const int64_t per = max(static_cast<int64_t>(A.min_tiles), (h.total + shares - 1) / shares), at = (blockIdx.x + 1) * per;
   const int block = find_block(T, h.blocks, h.total, at, &found);
   if (block < 0) return;
